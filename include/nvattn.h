@@ -224,6 +224,63 @@ NVATTN_API int nvattn_paged_decode_noalloc(const void* q, int64_t q_stride_tok, 
                                 int32_t* status, void* stream);
 
 /*
+ * The KV cache in 8-bit floating point (no counterpart in the reference, whose
+ * cache holds the model's type): the same pages at half the bytes.
+ *
+ *   k_cache, v_cache  [num_blocks][block_size][num_kv_heads][128] e4m3 bytes
+ *   k_scale, v_scale  [num_blocks][num_kv_heads][block_size] uint8: the row's
+ *                     scale 2^(byte - 127)
+ *
+ * A row is the 128 elements of one (token, KV head). With a its largest
+ * magnitude, the scale is the smallest power of two 2^k with a <= 448 * 2^k
+ * and k >= -100, and the elements are e4m3(x * 2^-k), rounded to nearest even;
+ * elements below 2^-10 * 2^k round to zero. A row that holds a value that is
+ * not finite is stored with byte 255 and NaN elements.
+ *
+ * nvattn_store_kvcache_fp8 quantises rows as nvattn_store_kvcache scatters
+ * them (same key/value views, slots and slot checks; slots other than -1 must
+ * be distinct within a call, or a row may end up with another row's scale).
+ *
+ * nvattn_load_kvcache_fp8 reads sequences back as the dense bf16 rows that
+ * nvattn_varlen_prefill takes (exactly: elements times 2^k): sequence b's key
+ * j goes to row cu_seqlens_k[b] + j of k_out and v_out [total_k]
+ * [num_kv_heads][128]. Rows outside [cu_seqlens_k[0], cu_seqlens_k[num_seqs])
+ * are left as they were, or zeroed with zero_rest != 0 (a dense prefill reads
+ * up to 127 rows behind a sequence's keys, masked: they must be finite); keys
+ * whose block id or table column is out of range
+ * become zeros and set NVATTN_STATUS_BAD_BLOCK. cu_seqlens_k must not decrease.
+ *
+ * nvattn_paged_decode_fp8 is nvattn_paged_decode over these caches, with the
+ * same sizes, limits and workspace (nvattn_decode_workspace_bytes); scores and
+ * sums are fp32 and the output is rounded to bf16 once. Scales must be 16-byte
+ * aligned.
+ */
+NVATTN_API int nvattn_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
+                                        int64_t value_stride, void* k_cache, void* v_cache,
+                                        uint8_t* k_scale, uint8_t* v_scale,
+                                        const int32_t* slot_mapping, int64_t num_tokens,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
+                                        int32_t block_size, int32_t* status, void* stream);
+
+NVATTN_API int nvattn_load_kvcache_fp8(const void* k_cache, const void* v_cache,
+                                       const uint8_t* k_scale, const uint8_t* v_scale,
+                                       const int32_t* cu_seqlens_k, int32_t num_seqs,
+                                       const int32_t* block_table, int64_t block_table_stride,
+                                       int32_t max_blocks_per_seq, int32_t num_blocks,
+                                       int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                                       int64_t total_k, int32_t zero_rest, void* k_out, void* v_out,
+                                       int32_t* status, void* stream);
+
+NVATTN_API int nvattn_paged_decode_fp8(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, const uint8_t* k_scale, const uint8_t* v_scale, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, const int32_t* cache_seqlens,
+    const int32_t* block_table, int64_t block_table_stride, int32_t max_blocks_per_seq,
+    int32_t num_blocks, int32_t block_size, int32_t batch, int32_t num_heads, int32_t num_kv_heads,
+    int32_t head_dim, float softmax_scale, void* workspace, size_t workspace_bytes,
+    int32_t* status, void* stream);
+
+/*
  * Tree-verification attention (no counterpart in the reference: EAGLE3-style
  * speculative verification, new in this library).
  *

@@ -25,18 +25,13 @@
 #include <cstdio>
 #include <mutex>
 
-#include "common.cuh"
+#include "decode.cuh"
 
 namespace nvattn {
 
-constexpr int kTile = 64;                      // tokens per pipeline stage
 constexpr int kDecStages = 3;                  // ring depth
 constexpr int kHalfBytes = kTile * 128;        // one 64-token x 64-dim half tile (8 KB)
 constexpr int kStageBytes = 4 * kHalfBytes;    // K lo/hi + V lo/hi (32 KB)
-constexpr int kDecConsumerWarps = 4;
-constexpr int kDecThreads = (kDecConsumerWarps + 1) * 32;
-constexpr int kMaxGroup = 16;                  // query heads per KV head handled per CTA
-constexpr int kOPad = 132;                     // fp32 row pitch of the merge buffer
 // Split policy (see choose_split); overridable at build time for tuning sweeps.
 #ifndef NVATTN_DEC_MIN_SPLIT_TILES
 #define NVATTN_DEC_MIN_SPLIT_TILES 4
@@ -46,25 +41,6 @@ constexpr int kOPad = 132;                     // fp32 row pitch of the merge bu
 #endif
 constexpr int kMinSplitTiles = NVATTN_DEC_MIN_SPLIT_TILES;
 constexpr int kSplitCtasPerSm = NVATTN_DEC_SPLIT_CTAS_PER_SM;
-
-struct DecodeParams {
-  const __nv_bfloat16* q;
-  int64_t q_stride_tok, q_stride_head;
-  __nv_bfloat16* out;
-  int64_t o_stride_tok, o_stride_head;
-  const int32_t* seqlens;
-  const int32_t* block_table;
-  int64_t bt_stride;
-  int32_t num_blocks, block_size, num_heads, num_kv_heads, group;
-  int32_t max_blocks;  // block-table width: keys past max_blocks*block_size are ignored
-  int32_t nsplit, split_tiles;
-  float scale_log2;
-  float* ws_o;    // [batch][num_heads][nsplit][128]
-  float2* ws_ml;  // [batch][num_heads][nsplit]  (running max (log2 units), sum)
-  int32_t* status;
-};
-
-__device__ __forceinline__ float neg_inf() { return -INFINITY; }
 
 __global__ void __launch_bounds__(kDecThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -383,8 +359,8 @@ static int device_sm_count() {
 // partials the combine reads; when one split covers the table, the kernel
 // writes the output itself and no combine runs).
 // Depends only on host-side sizes, so a captured graph keeps its grid.
-static void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size,
-                         int* nsplit, int* split_tiles) {
+void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size, int* nsplit,
+                  int* split_tiles) {
   const int sms = device_sm_count();
   const int64_t max_tiles = (static_cast<int64_t>(max_blocks) * block_size + kTile - 1) / kTile;
   const int64_t pairs = static_cast<int64_t>(batch) * num_kv_heads;
@@ -398,12 +374,36 @@ static void choose_split(int batch, int num_kv_heads, int max_blocks, int block_
   *nsplit = static_cast<int>(std::max<int64_t>(1, (max_tiles + st - 1) / st));
 }
 
-static size_t decode_ws_bytes(int batch, int num_heads, int nsplit) {
+size_t decode_ws_bytes(int batch, int num_heads, int nsplit) {
   if (nsplit <= 1) return 0;
   const size_t n = static_cast<size_t>(batch) * num_heads * nsplit;
   // partial O (128 fp32 per slot) followed by (max, sum) pairs; keep 256-B alignment.
   const size_t o_bytes = (n * kHeadDim * sizeof(float) + 255) & ~static_cast<size_t>(255);
   return o_bytes + n * sizeof(float2);
+}
+
+void set_decode_workspace(DecodeParams* p, void* workspace, int batch) {
+  p->ws_o = nullptr;
+  p->ws_ml = nullptr;
+  if (workspace == nullptr) return;
+  const size_t n = static_cast<size_t>(batch) * p->num_heads * p->nsplit;
+  const size_t o_bytes = (n * kHeadDim * sizeof(float) + 255) & ~static_cast<size_t>(255);
+  p->ws_o = static_cast<float*>(workspace);
+  p->ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + o_bytes);
+}
+
+static int launch_decode_combine(const DecodeParams& p, int batch, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.num_heads, batch);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_combine_kernel, p);
+  return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "decode_combine launch");
 }
 
 static int set_smem_attr(const void* fn, int bytes) {
@@ -433,30 +433,30 @@ int make_cache_map(CUtensorMap* map, const void* cache, int num_blocks, int bloc
   return make_tensor_map(map, cache, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Argument checks shared by both decode entry points (a negative batch is an
-// error; the caller handles batch == 0 before).
-static int check_decode_args(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
-                             const void* k_cache, const void* v_cache, const void* out,
-                             const int32_t* cache_seqlens, const int32_t* block_table,
-                             int64_t block_table_stride, int32_t max_blocks_per_seq,
-                             int32_t num_blocks, int32_t block_size, int32_t batch,
-                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
-  if (batch < 0) return fail(NVATTN_ERR_INVALID, "paged_decode: negative batch");
+// A negative batch is an error; the caller handles batch == 0 before.
+int check_decode_args(const char* who, const void* q, int64_t q_stride_tok,
+                      int64_t q_stride_head, const void* k_cache, const void* v_cache, const void* out,
+                      const int32_t* cache_seqlens, const int32_t* block_table,
+                      int64_t block_table_stride, int32_t max_blocks_per_seq,
+                      int32_t num_blocks, int32_t block_size, int32_t batch,
+                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
+  const auto msg = [who](const char* what) { return std::string(who) + ": " + what; };
+  if (batch < 0) return fail(NVATTN_ERR_INVALID, msg("negative batch"));
   if (!q || !k_cache || !v_cache || !out || !cache_seqlens || !block_table)
-    return fail(NVATTN_ERR_INVALID, "paged_decode: NULL pointer");
-  if (head_dim != kHeadDim) return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode: head_dim must be 128");
+    return fail(NVATTN_ERR_INVALID, msg("NULL pointer"));
+  if (head_dim != kHeadDim) return fail(NVATTN_ERR_UNSUPPORTED, msg("head_dim must be 128"));
   if (num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads)
-    return fail(NVATTN_ERR_INVALID, "paged_decode: num_heads must be a multiple of num_kv_heads");
+    return fail(NVATTN_ERR_INVALID, msg("num_heads must be a multiple of num_kv_heads"));
   if (num_heads / num_kv_heads > kMaxGroup)
-    return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode: more than 16 query heads per KV head");
+    return fail(NVATTN_ERR_UNSUPPORTED, msg("more than 16 query heads per KV head"));
   if (block_size <= 0 || block_size % kTile)
-    return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode: block_size must be a multiple of 64");
+    return fail(NVATTN_ERR_UNSUPPORTED, msg("block_size must be a multiple of 64"));
   if (num_blocks <= 0 || max_blocks_per_seq <= 0 || block_table_stride < max_blocks_per_seq)
-    return fail(NVATTN_ERR_INVALID, "paged_decode: bad block table geometry");
+    return fail(NVATTN_ERR_INVALID, msg("bad block table geometry"));
   if (!aligned16(k_cache) || !aligned16(v_cache))
-    return fail(NVATTN_ERR_INVALID, "paged_decode: caches must be 16-byte aligned");
+    return fail(NVATTN_ERR_INVALID, msg("caches must be 16-byte aligned"));
   if ((reinterpret_cast<uintptr_t>(q) & 3) || (q_stride_tok & 1) || (q_stride_head & 1))
-    return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode: q rows must be 4-byte aligned");
+    return fail(NVATTN_ERR_UNSUPPORTED, msg("q rows must be 4-byte aligned"));
   return NVATTN_OK;
 }
 
@@ -486,7 +486,7 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
                                    int32_t* status, void* stream) {
   clear_error();
   if (batch == 0) return NVATTN_OK;
-  int rc = check_decode_args(q, q_stride_tok, q_stride_head, k_cache, v_cache, out,
+  int rc = check_decode_args("paged_decode", q, q_stride_tok, q_stride_head, k_cache, v_cache, out,
                              cache_seqlens, block_table, block_table_stride, max_blocks_per_seq,
                              num_blocks, block_size, batch, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
@@ -525,17 +525,10 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
   p.max_blocks = max_blocks_per_seq;
   p.nsplit = nsplit;
   p.split_tiles = split_tiles;
+  p.key_begin = 0;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;
-  if (need > 0) {
-    const size_t n = static_cast<size_t>(batch) * num_heads * nsplit;
-    const size_t o_bytes = (n * kHeadDim * sizeof(float) + 255) & ~static_cast<size_t>(255);
-    p.ws_o = static_cast<float*>(workspace);
-    p.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + o_bytes);
-  } else {
-    p.ws_o = nullptr;
-    p.ws_ml = nullptr;
-  }
+  set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
 
   const int smem = kDecStages * kStageBytes + 1024 + 2 * kDecStages * 8 +
                    kDecConsumerWarps * kMaxGroup * 2 * 4;
@@ -547,20 +540,7 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
   paged_decode_kernel<<<grid, kDecThreads, smem, s>>>(kmap, vmap, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_decode launch");
-  if (nsplit > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_heads, batch);
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, decode_combine_kernel, p);
-    if (e != cudaSuccess) return cuda_fail(e, "decode_combine launch");
-  }
-  return NVATTN_OK;
+  return nsplit > 1 ? launch_decode_combine(p, batch, s) : NVATTN_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -619,7 +599,7 @@ extern "C" int nvattn_paged_decode_noalloc(
   if (batch == 0) return NVATTN_OK;
   // The same argument checks as nvattn_paged_decode come first, so a bad call
   // gets the same error from both entry points.
-  const int bad = check_decode_args(q, q_stride_tok, q_stride_head, k_cache, v_cache, out,
+  const int bad = check_decode_args("paged_decode", q, q_stride_tok, q_stride_head, k_cache, v_cache, out,
                                     cache_seqlens, block_table, block_table_stride,
                                     max_blocks_per_seq, num_blocks, block_size, batch, num_heads,
                                     num_kv_heads, head_dim);

@@ -10,15 +10,16 @@ from .attention import Attention
 from .context import Context, get_context, reset_context, set_context
 from . import ops, tree, parallel, decode_meta
 from .decode_meta import DecodeMetadata
-from .ops import (flash_attn_varlen_func, flash_attn_with_kvcache, kv_move, paged_decode,
-                  qk_norm_rope_store, sample, sample_merge, sample_shard, store_kvcache,
-                  tree_attention, varlen_prefill)
+from .ops import (flash_attn_varlen_func, flash_attn_with_kvcache, kv_move, load_kvcache_fp8,
+                  paged_decode, paged_decode_fp8, qk_norm_rope_store, sample, sample_merge,
+                  sample_shard, store_kvcache, store_kvcache_fp8, tree_attention, varlen_prefill)
 
 __all__ = [
     "Attention", "Context", "get_context", "set_context", "reset_context", "ops", "tree",
     "parallel", "store_kvcache", "varlen_prefill", "paged_decode", "tree_attention", "kv_move",
     "flash_attn_varlen_func", "flash_attn_with_kvcache", "qk_norm_rope_store", "sample",
-    "sample_shard", "sample_merge", "DecodeMetadata", "decode_meta", "install",
+    "sample_shard", "sample_merge", "store_kvcache_fp8", "load_kvcache_fp8", "paged_decode_fp8",
+    "DecodeMetadata", "decode_meta", "install",
 ]
 
 

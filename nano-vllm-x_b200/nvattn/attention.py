@@ -18,6 +18,11 @@ takes the raw q/k/v split of the QKV projection plus the RMSNorm weights and
 the rotary cache, and one kernel applies q_norm/k_norm and the rotation and
 scatters K/V (qwen3.py:82-86 and attention.py:62-63) before the attention.
 
+The cache may also be bound as ``float8_e4m3fn`` pages with their exponent
+bytes in ``k_scale``/``v_scale`` (``ops.store_kvcache_fp8``): new rows are then
+quantised as they are scattered, decode attends the fp8 pages, and a
+prefix-cache prefill reads its sequences back as dense bf16 rows first.
+
 All steps run libnvattn kernels; there is no other code path.
 """
 from __future__ import annotations
@@ -41,13 +46,24 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_scale = self.v_scale = None  # exponent bytes of an fp8 cache
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
         context = self.get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
         if k_cache.numel() and v_cache.numel():
-            ops.store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
+            self._store(k, v, context.slot_mapping)
         return self._attend(context, q, k, v)
+
+    def _fp8(self) -> bool:
+        return self.k_cache.dtype == torch.float8_e4m3fn
+
+    def _store(self, k, v, slot_mapping):
+        if self._fp8():
+            ops.store_kvcache_fp8(k, v, self.k_cache, self.v_cache, self.k_scale, self.v_scale,
+                                  slot_mapping)
+        else:
+            ops.store_kvcache(k, v, self.k_cache, self.v_cache, slot_mapping)
 
     def forward_fused(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                       v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -64,6 +80,11 @@ class Attention(nn.Module):
         # the rotated K itself is read only by dense prefill; the other paths
         # read K back from the cache
         need_k = bool(context.is_prefill and context.block_tables is None)
+        if bound and self._fp8():  # the kernel scatters bf16 rows: quantise its K after it
+            q, k = ops.qk_norm_rope_store(positions, q, k, v, q_weight, k_weight, cos_sin_cache,
+                                          eps)
+            self._store(k, v, context.slot_mapping)
+            return self._attend(context, q, k, v)
         q, k = ops.qk_norm_rope_store(positions, q, k, v, q_weight, k_weight, cos_sin_cache, eps,
                                       k_cache if bound else None, v_cache if bound else None,
                                       context.slot_mapping if bound else None, need_k=need_k)
@@ -72,12 +93,26 @@ class Attention(nn.Module):
     def _attend(self, context, q: torch.Tensor, k, v):
         k_cache, v_cache = self.k_cache, self.v_cache
         if context.is_prefill:
-            if context.block_tables is not None:  # prefix cache
+            block_table = context.block_tables
+            if block_table is not None:  # prefix cache
                 k, v = k_cache, v_cache
+                if self._fp8():
+                    # no sequence has more keys than its table holds or than
+                    # max_seqlen_k: an upper bound of cu_seqlens_k[-1] without
+                    # reading it back from the device
+                    total_k = block_table.shape[0] * min(context.max_seqlen_k,
+                                                         block_table.shape[1] * k_cache.shape[1])
+                    k, v = ops.load_kvcache_fp8(k_cache, v_cache, self.k_scale, self.v_scale,
+                                                context.cu_seqlens_k, block_table, total_k)
+                    block_table = None
             o = ops.varlen_prefill(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
                                    context.max_seqlen_q, context.max_seqlen_k,
                                    softmax_scale=self.scale, causal=True,
-                                   block_table=context.block_tables)
+                                   block_table=block_table)
+        elif self._fp8():
+            o = ops.paged_decode_fp8(q, k_cache, v_cache, self.k_scale, self.v_scale,
+                                     context.context_lens, context.block_tables,
+                                     softmax_scale=self.scale).unsqueeze(1)
         else:  # decode
             o = ops.paged_decode(q, k_cache, v_cache, context.context_lens,
                                  context.block_tables, softmax_scale=self.scale).unsqueeze(1)

@@ -17,6 +17,9 @@ on a machine without the CUDA library these functions raise.
     sample_shard,            the same pick per vocabulary shard and the merge
     sample_merge             of the shards' keys, in place of ParallelLMHead's
                              logits gather at TP > 1 (embed_head.py:56-66)
+    store_kvcache_fp8,       new: the cache in 8-bit floating point — scatter
+    load_kvcache_fp8,        with quantisation, read back as dense bf16 rows,
+    paged_decode_fp8         decode attention over it
 
 Every launch is asynchronous on ``torch.cuda.current_stream()``, performs
 no host synchronisation and allocates only through torch's caching
@@ -24,6 +27,8 @@ allocator, so the decode path can be captured in a CUDA graph the way
 ``ModelRunner.capture_cudagraph`` (model_runner.py:222-257) does.
 """
 from __future__ import annotations
+
+import contextlib
 
 import torch
 
@@ -37,6 +42,9 @@ __all__ = [
     "paged_decode",
     "tree_attention",
     "kv_move",
+    "store_kvcache_fp8",
+    "load_kvcache_fp8",
+    "paged_decode_fp8",
     "qk_norm_rope_store",
     "sample",
     "sample_shard",
@@ -113,6 +121,14 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _device(device: torch.device):
+    """Makes `device` current for a launch (nothing to do when it already is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _check_bf16(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and t.dtype != torch.bfloat16:
@@ -124,6 +140,49 @@ def _check_i32(name: str, t: torch.Tensor) -> None:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _check_table(block_table: torch.Tensor, rows: int) -> None:
+    """An int32 (rows, W) block table; rows may be strided (a slice of a wider table)."""
+    if block_table.dtype != torch.int32:
+        raise TypeError(f"block_table must be int32, got {block_table.dtype}")
+    if block_table.dim() != 2 or block_table.shape[0] != rows:
+        raise ValueError("block_table needs one row per sequence")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError("block_table rows must be contiguous")
+
+
+def _check_decode(q: torch.Tensor, out: torch.Tensor | None, cache_seqlens: torch.Tensor,
+                  block_table: torch.Tensor, num_kv_heads: int, cache_dim: int):
+    """Argument checks of the decode operators; returns (batch, heads, d, out)."""
+    _check_bf16(q, out)
+    _check_i32("cache_seqlens", cache_seqlens)
+    if q.dim() != 3:
+        raise ValueError("q must be (batch, num_heads, head_dim)")
+    batch, num_heads, head_dim = q.shape
+    _check_table(block_table, batch)
+    if q.stride(2) != 1:
+        raise ValueError("q must have a contiguous last dimension")
+    if cache_dim != head_dim:
+        raise ValueError("q and cache head_dim differ")
+    if num_heads % num_kv_heads:
+        raise ValueError("num_heads must be a multiple of num_kv_heads")
+    if cache_seqlens.numel() != batch:
+        raise ValueError("cache_seqlens must have one entry per row of q")
+    if out is None:
+        out = torch.empty((batch, num_heads, head_dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and a contiguous last dimension")
+    return batch, num_heads, head_dim, out
+
+
+def _workspace(need: int, workspace: torch.Tensor | None, device: torch.device):
+    """(pointer, bytes) of the caller's workspace, or of a new one of `need` bytes."""
+    if not need:
+        return None, 0
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 # --------------------------------------------------------------------- scatter
@@ -307,6 +366,127 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, cache_seqlens=None, block_table
                        cu_k, seqlen_q, max_k, softmax_scale=softmax_scale, causal=causal,
                        block_table=block_table)
     return o.view(batch, seqlen_q, num_heads, head_dim)
+
+
+# ------------------------------------------------------------------- fp8 cache
+
+def _check_fp8_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                      v_scale: torch.Tensor) -> tuple[int, int, int]:
+    """Shapes of an fp8 cache and its exponents; returns (num_blocks, block_size, kv_heads)."""
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError("fp8 caches must be float8_e4m3fn, got "
+                        f"{k_cache.dtype} and {v_cache.dtype}")
+    if k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
+        raise TypeError("k_scale and v_scale must be uint8 exponent bytes")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
+        raise ValueError("caches must be (num_blocks, block_size, kv_heads, d)")
+    num_blocks, block_size, num_kv_heads, _ = shape
+    if k_scale.shape != (num_blocks, num_kv_heads, block_size) or v_scale.shape != k_scale.shape:
+        raise ValueError("k_scale and v_scale must be (num_blocks, kv_heads, block_size)")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise ValueError("fp8 caches and their scales must be contiguous")
+    return num_blocks, block_size, num_kv_heads
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                      slot_mapping: torch.Tensor) -> None:
+    """``store_kvcache`` into an fp8 cache, quantising each (token, KV head) row.
+
+    key, value: (N, KVH, 128) bf16 with contiguous tokens, as in
+    ``store_kvcache``; k_cache, v_cache: (num_blocks, block_size, KVH, 128)
+    float8_e4m3fn; k_scale, v_scale: (num_blocks, KVH, block_size) uint8. A
+    row's elements are e4m3(x / 2^k), its byte k + 127, with 2^k the smallest
+    power of two (k >= -100) that brings the row's largest magnitude to at
+    most 448; a row with a value that is not finite reads back as NaN. Slot -1
+    is skipped; the other slots of a call must be distinct.
+    """
+    N, num_heads, head_dim = key.shape
+    dev = _require_cuda(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    _check_bf16(key, value)
+    _check_i32("slot_mapping", slot_mapping)
+    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    if value.shape != key.shape or (num_heads, head_dim) != (num_kv_heads, k_cache.shape[3]):
+        raise ValueError("key/value must be (N, kv_heads, d) like the caches' rows")
+    for n, t in (("key", key), ("value", value)):
+        if t.stride(2) != 1 or (num_heads > 1 and t.stride(1) != head_dim):
+            raise ValueError(f"{n} must have unit element stride and head stride head_dim")
+    if slot_mapping.numel() != N:
+        raise ValueError("slot_mapping must have one entry per token")
+    with _device(dev):
+        _lib.call("nvattn_store_kvcache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(),
+                  value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                  v_scale.data_ptr(), slot_mapping.data_ptr(), N, num_kv_heads, head_dim,
+                  num_blocks, block_size, _status_ptr(dev), _stream(dev))
+
+
+def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, cu_seqlens_k: torch.Tensor, block_table: torch.Tensor,
+                     total_k: int, k_out: torch.Tensor | None = None,
+                     v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Sequences of an fp8 cache as dense bf16 (total_k, KVH, 128) keys and values,
+    the dense input of ``varlen_prefill``.
+
+    Key j of sequence b (cu_seqlens_k (S + 1,), block_table (S, W), both
+    int32) lands in row cu_seqlens_k[b] + j; rows behind the last sequence are
+    left as they were in a given k_out and v_out, and zeros in new ones.
+    """
+    dev = _require_cuda(k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_table, k_out,
+                        v_out)
+    _check_i32("cu_seqlens_k", cu_seqlens_k)
+    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    num_seqs = cu_seqlens_k.numel() - 1
+    _check_table(block_table, num_seqs)
+    head_dim = k_cache.shape[3]
+    shape = (int(total_k), num_kv_heads, head_dim)
+    new = k_out is None
+    if new != (v_out is None):
+        raise ValueError("give both k_out and v_out, or neither")
+    if new:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    _check_bf16(k_out, v_out)
+    for n, t in (("k_out", k_out), ("v_out", v_out)):
+        if t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{n} must be contiguous {shape}")
+    with _device(dev):
+        _lib.call("nvattn_load_kvcache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
+                  k_scale.data_ptr(), v_scale.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs,
+                  block_table.data_ptr(), block_table.stride(0), block_table.shape[1], num_blocks,
+                  block_size, num_kv_heads, head_dim, int(total_k), 1 if new else 0, k_out.data_ptr(),
+                  v_out.data_ptr(), _status_ptr(dev), _stream(dev))
+    return k_out, v_out
+
+
+def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     k_scale: torch.Tensor, v_scale: torch.Tensor, cache_seqlens: torch.Tensor,
+                     block_table: torch.Tensor, softmax_scale: float | None = None,
+                     out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_decode`` over an fp8 cache (``store_kvcache_fp8``); q, out: (B, H, d) bf16.
+
+    ``workspace``: uint8, ``decode_workspace_bytes`` of the same sizes.
+    """
+    dev = _require_cuda(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, out,
+                        workspace)
+    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    batch, num_heads, head_dim, out = _check_decode(q, out, cache_seqlens, block_table,
+                                                    num_kv_heads, k_cache.shape[3])
+    max_blocks = block_table.shape[1]
+    with _device(dev):
+        ws_ptr, ws_bytes = _workspace(decode_workspace_bytes(batch, num_heads, num_kv_heads,
+                                                             max_blocks, block_size),
+                                      workspace, dev)
+        _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
+                  k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),
+                  block_table.data_ptr(), block_table.stride(0), max_blocks, num_blocks,
+                  block_size, batch, num_heads, num_kv_heads, head_dim,
+                  head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
+                  ws_bytes, _status_ptr(dev), _stream(dev))
+    return out
 
 
 # ------------------------------------------------------------------------ tree

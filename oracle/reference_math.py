@@ -493,3 +493,68 @@ def merge_pick_keys(keys: np.ndarray) -> np.ndarray:
     k = np.asarray(keys, np.uint64).max(axis=0)
     col = (np.uint64(0xFFFFFFFF) - (k & np.uint64(0xFFFFFFFF))).astype(np.int64)
     return np.where(k != 0, col, 0)
+
+
+# ---------------------------------------------------------------- fp8 KV cache
+
+def quantise_rows_fp8(x: torch.Tensor):
+    """Rows (..., 128) -> (float8_e4m3fn elements, uint8 exponent bytes (...)):
+    the smallest power of two 2^k, k >= -100, with max|x| <= 448 * 2^k, found by
+    counting up in exact arithmetic; byte k + 127; a row that is not finite is
+    NaN with byte 255."""
+    x = x.double()
+    amax = x.abs().amax(-1)
+    k = torch.full(amax.shape, -100, dtype=torch.int64)
+    for e in range(-100, 121):  # 448 * 2^e is exact in fp64
+        k = torch.where(amax > 448.0 * 2.0 ** e, e + 1, k)
+    bad = ~torch.isfinite(amax)
+    k = torch.where(bad, 0, k)
+    q = (x * torch.exp2(-k.double())[..., None]).float().to(torch.float8_e4m3fn)
+    q = torch.where(bad[..., None], torch.full(x.shape, 0x7F, dtype=torch.uint8),
+                    q.view(torch.uint8))
+    return q.view(torch.float8_e4m3fn), torch.where(bad, 255, k + 127).to(torch.uint8)
+
+
+def expand_rows_fp8(q: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
+    """fp64 values of quantised rows (NaN where the byte is 255)."""
+    s = torch.exp2(byte.double() - 127.0)
+    return q.float().double() * torch.where(byte == 255, torch.nan, s)[..., None]
+
+
+def expand_cache_fp8(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """fp64 values of a whole fp8 cache (num_blocks, block_size, KVH, 128) with
+    its exponents (num_blocks, KVH, block_size)."""
+    return expand_rows_fp8(cache, scale.transpose(1, 2))
+
+
+def decode_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_seqlens,
+                         block_table, scale: float, shared_len: int = 0):
+    """One query per sequence in fp64 over caches of values (num_blocks,
+    block_size, KVH, d); with shared_len, keys below it come through row 0 of
+    the table. Returns (out (B, H, d), a dict of per-(row, head) magnitudes
+    that error bounds need): ``mix`` (B, H, d) = sum_j p_j |v_j|, ``dot``
+    (B, H) = the largest sum_d |q_d k_d| * scale, ``n`` (B, H) keys."""
+    B, H, d = q.shape
+    bs, KVH = k.shape[1], k.shape[2]
+    G = H // KVH
+    out = torch.zeros(B, H, d, dtype=torch.float64)
+    mag = dict(mix=torch.zeros_like(out), dot=torch.zeros(B, H, dtype=torch.float64),
+               n=torch.zeros(B, H, dtype=torch.float64))
+    table = torch.as_tensor(np.asarray(block_table)).long()
+    k, v = k.double(), v.double()
+    for b, n in enumerate(int(x) for x in cache_seqlens):
+        if n <= 0:
+            continue
+        pos = torch.arange(n)
+        row = torch.where(pos < shared_len, 0, b)
+        blk = table[row, pos // bs]
+        kb, vb = k[blk, pos % bs], v[blk, pos % bs]
+        for h in range(H):
+            g = h // G
+            prod = kb[:, g] * q[b, h].double()
+            p = torch.softmax(prod.sum(-1) * scale, 0)
+            out[b, h] = p @ vb[:, g]
+            mag["mix"][b, h] = p @ vb[:, g].abs()
+            mag["dot"][b, h] = prod.abs().sum(-1).max() * scale
+            mag["n"][b, h] = n
+    return out, mag
