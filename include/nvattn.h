@@ -403,6 +403,48 @@ NVATTN_API int nvattn_sample_merge(const uint64_t* keys, int64_t num_shards, int
                                    int64_t* out_tokens, void* stream);
 
 /*
+ * Verification of drafted tokens against the target's probabilities, from
+ * given random numbers (no counterpart in the reference): which drafts stand,
+ * and the token that follows them.
+ *
+ * logits [batch][nodes][vocab] bf16 (strides in elements between sequences
+ * and rows): row j of a sequence is the target's answer after node j. Node 0
+ * is the last committed token; node j > 0 is the drafted token
+ * draft_tokens[b][j-1] with parent parents[b * parents_stride + j] (< j;
+ * parents NULL: a chain, the parent of j is j - 1). num_nodes (nullable) limits
+ * sequence b to its first num_nodes[b] nodes; 0 marks a padding row.
+ * With p = softmax(logits / temperature), the walk goes from node 0; at a node
+ * its children are tried in order:
+ *   draft_logits NULL: child c is accepted iff u_accept[b][c-1] * R < p(token),
+ *     R = 1 - the sum of p over the siblings' tokens rejected before (a token
+ *     tried before counts as p = 0); if none is accepted, the next token is
+ *     drawn from p without the rejected tokens;
+ *   draft_logits [batch][nodes-1][vocab] (chains only), q = softmax(draft_logits
+ *     row of the node / temperature): accepted iff u * q(token) < p(token),
+ *     else the next token is drawn from max(p - q, 0);
+ * and where a node has no child the next token is drawn from p. Either way the
+ * tokens follow the target's law. The draw takes the first column whose
+ * cumulative weight exceeds u_pick[b] * total, in column order; where rounding
+ * leaves no weight it is from p. temperatures NULL or <= 0: greedy, a child is
+ * accepted iff its token is the argmax (first index on ties), which is also the
+ * draw. NaN and -inf logits have no probability, an infinite one all of it; a
+ * row with nothing else accepts nothing and gives column 0. A drafted token
+ * outside [0, vocab) is rejected. Decisions are those of 64-bit arithmetic.
+ *
+ * out_num[b] = number of accepted drafts a; out_path[b][0..a] = the walked
+ * nodes from 0; out_tokens[b][0..a-1] = the accepted tokens, out_tokens[b][a] =
+ * the drawn one; -1 behind them (everywhere, with out_num 0, in a padding row).
+ * draft_tokens, u_accept (batch, nodes - 1), out_tokens and out_path (batch,
+ * nodes) are contiguous. nodes <= 64, vocab <= 393216.
+ */
+NVATTN_API int nvattn_verify_draft(
+    const void* logits, int64_t l_stride_seq, int64_t l_stride_row, const void* draft_logits,
+    int64_t d_stride_seq, int64_t d_stride_row, const int64_t* draft_tokens,
+    const int32_t* parents, int64_t parents_stride, const float* u_accept, const float* u_pick,
+    const float* temperatures, const int32_t* num_nodes, int32_t batch, int32_t nodes,
+    int32_t vocab, int64_t* out_tokens, int32_t* out_path, int32_t* out_num, void* stream);
+
+/*
  * Decode-step metadata from one packed host record per sequence.
  * packed layout (num_seqs = B, table_width = W, 8-byte aligned):
  *   int64 last_token[B] | int32 num_tokens[B] | int32 table_len[B] |

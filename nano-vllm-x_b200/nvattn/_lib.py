@@ -87,6 +87,9 @@ SIGNATURES: dict[str, tuple] = {
     "nvattn_sample_shard": (c_int, [_P, c_int64, c_int64, c_int64, c_int64, _P, c_uint64, c_uint64,
                                     _P, _P]),
     "nvattn_sample_merge": (c_int, [_P, c_int64, c_int64, _P, _P]),
+    "nvattn_verify_draft": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, _I32P, c_int64,
+                                    _P, _P, _P, _I32P, c_int32, c_int32, c_int32, _P, _I32P, _I32P,
+                                    _P]),
     "nvattn_ar_buffer_bytes": (c_size_t, [c_int64]),
     "nvattn_ar_alloc": (c_int, [c_size_t, _P, _P]),
     "nvattn_ar_open": (c_int, [_P, _P]),

@@ -20,6 +20,8 @@ on a machine without the CUDA library these functions raise.
     store_kvcache_fp8,       new: the cache in 8-bit floating point — scatter
     load_kvcache_fp8,        with quantisation, read back as dense bf16 rows,
     paged_decode_fp8         decode attention over it
+    verify_draft             new: which drafted tokens stand against the
+                             target's probabilities, and the token after them
 
 Every launch is asynchronous on ``torch.cuda.current_stream()``, performs
 no host synchronisation and allocates only through torch's caching
@@ -49,6 +51,7 @@ __all__ = [
     "sample",
     "sample_shard",
     "sample_merge",
+    "verify_draft",
     "decode_workspace_bytes",
     "tree_workspace_bytes",
     "status_tensor",
@@ -721,3 +724,69 @@ def sample_merge(keys: torch.Tensor, out: torch.Tensor | None = None) -> torch.T
         raise ValueError("keys must hold at least one shard")
     _lib.call("nvattn_sample_merge", keys.data_ptr(), S, B, out.data_ptr(), _stream(dev))
     return out
+
+
+# ---------------------------------------------------------------- verification
+
+def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: torch.Tensor,
+                 u_pick: torch.Tensor, temperatures: torch.Tensor | None = None,
+                 draft_logits: torch.Tensor | None = None, parents: torch.Tensor | None = None,
+                 num_nodes: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Accepts drafted tokens against the target's probabilities and draws the next one.
+
+    logits: (B, n, V) bf16, row j the target's answer after node j (node 0 the
+    last committed token, node j > 0 drafted token ``draft_tokens[b, j - 1]``,
+    (B, n - 1) int64). ``parents`` (B, n) int32 makes the nodes a tree (``tree.
+    build_draft_tree`` order, every parent before its children; an expanded
+    (n,) row will do); without it they are a chain. ``draft_logits`` (B, n - 1,
+    V) bf16, for chains, are the draft model's rows that the tokens were drawn
+    from; without them the drafts count as proposed with certainty (greedy or
+    n-gram drafts). ``u_accept`` (B, n - 1) and ``u_pick`` (B,) are uniform
+    random numbers in [0, 1), fp32. ``temperatures`` (B,) fp32 as in ``sample``
+    (<= 0 or None: greedy). ``num_nodes`` (B,) int32: nodes in use per sequence
+    (0: a padding row).
+
+    Returns (tokens (B, n) int64: the accepted tokens, then the drawn one, then
+    -1; path (B, n) int32: the walked nodes from 0, then -1, for
+    ``tree.compaction_moves``; accepted (B,) int32). The tokens follow the
+    target's law; every decision is that of 64-bit arithmetic.
+    """
+    dev = _require_cuda(logits, draft_tokens, u_accept, u_pick, temperatures, draft_logits,
+                        parents, num_nodes)
+    _check_bf16(logits, draft_logits)
+    if logits.dim() != 3 or logits.stride(2) != 1:
+        raise ValueError("logits must be (B, n, V) with unit column stride")
+    B, n, V = logits.shape
+    if n < 1:
+        raise ValueError("logits needs at least the root's row")
+    for name, t, dtype, shape in (("draft_tokens", draft_tokens, torch.int64, (B, n - 1)),
+                                  ("u_accept", u_accept, torch.float32, (B, n - 1)),
+                                  ("u_pick", u_pick, torch.float32, (B,)),
+                                  ("temperatures", temperatures, torch.float32, (B,)),
+                                  ("num_nodes", num_nodes, torch.int32, (B,))):
+        if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {shape} {dtype} tensor")
+    if parents is not None and (parents.dtype != torch.int32 or parents.shape != (B, n)
+                                or (n > 1 and parents.stride(1) != 1)):
+        raise ValueError(f"parents must be a ({B}, {n}) int32 tensor with unit column stride")
+    d_strides = (0, 0)
+    if draft_logits is not None:
+        if parents is not None:
+            raise ValueError("draft_logits go with a chain: give no parents")
+        if draft_logits.shape != (B, n - 1, V) or (n > 1 and draft_logits.stride(2) != 1):
+            raise ValueError("draft_logits must be (B, n - 1, V) with unit column stride")
+        d_strides = draft_logits.stride()[:2]
+    tokens = torch.empty((B, n), dtype=torch.int64, device=dev)
+    path = torch.empty((B, n), dtype=torch.int32, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    with _device(dev):
+        _lib.call("nvattn_verify_draft", logits.data_ptr(), logits.stride(0), logits.stride(1),
+                  draft_logits.data_ptr() if draft_logits is not None and n > 1 else None,
+                  *d_strides, draft_tokens.data_ptr(),
+                  parents.data_ptr() if parents is not None else None,
+                  parents.stride(0) if parents is not None else 0, u_accept.data_ptr(),
+                  u_pick.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
+                  num_nodes.data_ptr() if num_nodes is not None else None, B, n, V,
+                  tokens.data_ptr(), path.data_ptr(), accepted.data_ptr(), _stream(dev))
+    return tokens, path, accepted

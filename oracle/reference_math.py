@@ -558,3 +558,79 @@ def decode_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cach
             mag["dot"][b, h] = prod.abs().sum(-1).max() * scale
             mag["n"][b, h] = n
     return out, mag
+
+
+# ------------------------------------------------------- draft verification
+
+def verify_law(row, temperature: float) -> np.ndarray:
+    """fp64 softmax(row / T), or the argmax's indicator for T <= 0; NaN and -inf
+    have none, +inf shares all; zeros when nothing has any."""
+    x = torch.as_tensor(row).double().numpy().copy()
+    x[np.isnan(x)] = -np.inf
+    top = x.max()
+    if top == -np.inf:
+        return np.zeros_like(x)
+    if not temperature > 0:
+        return (np.arange(x.size) == int(np.argmax(x))).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == top, 1.0, np.exp((x - top) / np.float64(np.float32(temperature))))
+    return w / w.sum()
+
+
+def verify_draw(w: np.ndarray, u: float) -> int:
+    """First column whose cumulative weight exceeds u * total (the last one with
+    weight when rounding leaves none)."""
+    c = np.cumsum(w)
+    over = np.nonzero(c > max(float(u), 0.0) * c[-1])[0]
+    return int(over[0]) if over.size else int(np.nonzero(w > 0)[0][-1])
+
+
+def verify_draft(logits, draft_tokens, u_accept, u_pick, temperatures=None, draft_logits=None,
+                 parents=None, num_nodes=None):
+    """The walk of nvattn_verify_draft, one sequence and one node after another;
+    returns (tokens, path, accepted) as numpy arrays."""
+    B, n, V = logits.shape
+    tokens = np.full((B, n), -1, np.int64)
+    path = np.full((B, n), -1, np.int32)
+    num = np.zeros(B, np.int32)
+    for b in range(B):
+        T = 0.0 if temperatures is None else float(temperatures[b])
+        live = n if num_nodes is None else min(max(int(num_nodes[b]), 0), n)
+        if live == 0:
+            continue
+        up = [-1] + list(range(n - 1)) if parents is None else [int(x) for x in parents[b]]
+        node, step = 0, 0
+        path[b, 0] = 0
+        while True:
+            p = verify_law(logits[b, node], T)
+            rest, left, found = p.copy(), 1.0, None
+            for c in range(node + 1, live):
+                if up[c] != node:
+                    continue
+                x, u = int(draft_tokens[b, c - 1]), float(u_accept[b, c - 1])
+                inside = 0 <= x < V
+                here = rest[x] if inside else 0.0
+                if draft_logits is not None and T > 0:
+                    q = verify_law(draft_logits[b, node], T)
+                    against = q[x] if inside else 0.0
+                    rest = np.maximum(p - q, 0.0)
+                    here = p[x] if inside else 0.0
+                else:
+                    against = left
+                if (here > 0 if not T > 0 else u * against < here) and here > 0:
+                    found = c
+                    break
+                if draft_logits is None and inside:
+                    left -= here
+                    rest[x] = 0.0
+            if found is None:
+                break
+            tokens[b, step] = int(draft_tokens[b, found - 1])
+            node, step = found, step + 1
+            path[b, step] = node
+        if not T > 0 or p.sum() == 0:
+            tokens[b, step] = int(np.argmax(p))
+        else:
+            tokens[b, step] = verify_draw(rest if rest.sum() > 0 else p, float(u_pick[b]))
+        num[b] = step
+    return tokens, path, num
