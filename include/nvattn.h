@@ -281,6 +281,40 @@ NVATTN_API int nvattn_paged_decode_fp8(
     int32_t* status, void* stream);
 
 /*
+ * Decode attention for a batch that shares a long prefix (no counterpart in
+ * the reference): nvattn_paged_decode, with the keys [0, shared_len) that all
+ * sequences have in common read and multiplied once for the whole batch.
+ *
+ * Their pages are the first shared_len / block_size entries of row 0 of
+ * block_table (rows with at least shared_len keys are taken to hold the same
+ * ids there); key j >= shared_len of sequence b comes through row b.
+ * cache_seqlens counts all keys of a sequence; a row with fewer than
+ * shared_len keys (0: a padding row, whose output is zeros) is attended over
+ * its own pages alone. shared_len is a multiple of block_size (0: none shared),
+ * block_size one of 128. k_scale and v_scale NULL: bf16 caches; otherwise fp8
+ * caches as for nvattn_paged_decode_fp8. q rows are 16-byte aligned.
+ *
+ * `workspace` (device, 256-byte aligned, >= nvattn_shared_prefix_workspace_bytes
+ * of the same sizes; fp8 = 0 or 1) holds fp32 partials of both parts and, for an
+ * fp8 cache, the prefix's bf16 rows. Sizes and splits depend on host-side
+ * arguments only, so a captured graph keeps its grids.
+ */
+NVATTN_API size_t nvattn_shared_prefix_workspace_bytes(int32_t batch, int32_t num_heads,
+                                                       int32_t num_kv_heads,
+                                                       int32_t max_blocks_per_seq,
+                                                       int32_t block_size, int32_t shared_len,
+                                                       int32_t fp8);
+
+NVATTN_API int nvattn_shared_prefix_decode(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, const uint8_t* k_scale, const uint8_t* v_scale, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, const int32_t* cache_seqlens,
+    const int32_t* block_table, int64_t block_table_stride, int32_t max_blocks_per_seq,
+    int32_t num_blocks, int32_t block_size, int32_t shared_len, int32_t batch, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, float softmax_scale, void* workspace,
+    size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
  * Tree-verification attention (no counterpart in the reference: EAGLE3-style
  * speculative verification, new in this library).
  *

@@ -41,10 +41,16 @@
 // written: a warp with no valid row skips its softmax entirely, and inside a
 // live warp such rows take the unmasked path (rows are independent in both
 // MMAs, so their values cannot reach a valid row).
+//
+// Shared mode (decode over a prefix that a whole batch shares,
+// shared_prefix.cu): the batch's rows are one sequence's query tokens, every
+// key of the prefix is visible to all of them, no tile is partial, and every
+// CTA writes fp32 partials of its split of the keys.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
 
+#include "shared_prefix.cuh"
 #include "sm100.cuh"
 
 namespace nvattn {
@@ -74,7 +80,7 @@ constexpr int kPolyEveryTree = 8;
 #endif
 constexpr int kPrefetch = NVATTN_L2_PREFETCH_TILES;  // key tiles of L2 prefetch ahead of the ring
 
-enum Mode { kDense = 0, kPaged = 1, kTree = 2 };
+enum Mode { kDense = 0, kPaged = 1, kTree = 2, kShared = 3 };
 
 
 struct Params {
@@ -104,6 +110,10 @@ struct Params {
   // Tree mode: sequences in decreasing key count (written by
   // tree_order_kernel), so CTAs are dispatched longest first; null = in order.
   const int32_t* order;
+  // Shared mode: the rows' key counts; rows with fewer keys than the prefix
+  // (padding among them) take no part. block_table null: pages in order.
+  const int32_t* seqlens;
+  int32_t shared_len;
 };
 
 struct Barriers {
@@ -152,20 +162,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr bool kSplitP = MODE == kTree;
   constexpr int kPolyEvery = MODE == kTree ? kPolyEveryTree : kPolyEveryPrefill;
 
+  if (MODE == kShared) {
+    // the kernel over the rows' own keys may start beside this one's last CTAs
+    asm volatile("griddepcontrol.launch_dependents;");
+  }
+
   // ------------------------------------------------ sequence geometry
-  const int q_begin = p.cu_q[b];
-  int Lq = p.cu_q[b + 1] - q_begin;
+  const int q_begin = MODE == kShared ? 0 : p.cu_q[b];
+  int Lq = MODE == kShared ? static_cast<int>(p.total_q) : p.cu_q[b + 1] - q_begin;
   if (q_begin < 0 || q_begin > p.total_q) return;
   if (q_begin + static_cast<int64_t>(Lq) > p.total_q) Lq = static_cast<int>(p.total_q - q_begin);
   int Lk, k_begin = 0, ctx = 0;
   if (MODE == kTree) {
     ctx = p.ctx_lens[b];
     Lk = ctx + Lq;
+  } else if (MODE == kShared) {
+    Lk = p.shared_len;
   } else {
     k_begin = p.cu_k[b];
     Lk = p.cu_k[b + 1] - k_begin;
   }
-  if (MODE != kDense && Lk > p.max_blocks * p.block_size) {
+  if (MODE != kDense && MODE != kShared && Lk > p.max_blocks * p.block_size) {
     if (blockIdx.x == 0 && threadIdx.x == 0) set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
     const int cut = Lk - p.max_blocks * p.block_size;
     Lk -= cut;
@@ -177,14 +194,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tok_hi = min(Lq - 1, tok0 + 2 * p.tpt - 1);
   const int diag = Lk - Lq;
   int kend;
-  if (MODE == kTree)
+  if (MODE == kTree || MODE == kShared)
     kend = Lk;
   else
     kend = p.causal ? min(Lk, diag + tok_hi + 1) : Lk;
   const int ntiles_all = kend > 0 ? (kend + kBN - 1) / kBN : 0;
   const int jb = split * p.split_tiles;  // first key tile of this CTA's split
   const int ntiles = max(0, min(ntiles_all, jb + p.split_tiles) - jb);
-  if (p.nsplit > 1 && ntiles == 0) return;  // split past the keys: the merge skips it
+  if ((MODE == kShared || p.nsplit > 1) && ntiles == 0)
+    return;  // split past the keys: the merge skips it
+  // Shared mode: a small batch leaves the second Q tile without rows
+  const bool two = MODE != kShared || tok0 + p.tpt < Lq;
 
   if (ntiles == 0) {
     // No visible key for any row of this CTA: the rows are zeros.
@@ -260,7 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (MODE == kDense) {
           c2 = k_begin + j0;
         } else {
-          int blk = bt[j0 / p.block_size];
+          int blk = (MODE == kShared && p.block_table == nullptr) ? j0 / p.block_size
+                                                                  : bt[j0 / p.block_size];
           if (blk < 0 || blk >= p.num_blocks) {
             set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
             blk = 0;
@@ -279,7 +300,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch_3d(&vmap, 0, g, pc2);
             tma_prefetch_3d(&vmap, 64, g, pc2);
           } else {
-            const int pblk = bt[pj0 / p.block_size];
+            const int pblk = (MODE == kShared && p.block_table == nullptr)
+                                 ? pj0 / p.block_size
+                                 : bt[pj0 / p.block_size];
             if (pblk >= 0 && pblk < p.num_blocks) {
               const int pc2 = pj0 % p.block_size;
               tma_prefetch_4d(&kmap, 0, g, pc2, pblk);
@@ -344,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) {
         sm100::fence_after_sync();
         issue_s(0, 0);
-        issue_s(1, 0);
+        if (two) issue_s(1, 0);
         sm100::commit(&bars->k_empty[0]);
       }
       for (int j = 0; ok && j < ntiles; ++j) {
@@ -380,13 +403,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm100::fence_after_sync();
           issue_pv(1, st, j, 0, 4);
         }
-        ok = mbar_wait(&bars->p_full[1], j & 1);
-        if (!ok) break;
-        sm100::fence_after_sync();
-        issue_pv(1, st, j, kSplitP ? 4 : 0, 8);
+        if (two) {
+          ok = mbar_wait(&bars->p_full[1], j & 1);
+          if (!ok) break;
+          sm100::fence_after_sync();
+          issue_pv(1, st, j, kSplitP ? 4 : 0, 8);
+        }
         sm100::commit(&bars->v_empty[st]);
         if (more) {
-          issue_s(1, nst);
+          if (two) issue_s(1, nst);
           sm100::commit(&bars->k_empty[nst]);
         }
       }
@@ -403,8 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const int tok = tok0 + wg * p.tpt + r / group;
     const int hh = r % group;
-    const bool valid = r < p.rpt && tok < Lq;
-    const int lim = valid ? ((MODE != kTree && p.causal) ? min(Lk - 1, diag + tok) : Lk - 1) : -1;
+    const bool valid = r < p.rpt && tok < Lq &&
+                       (MODE != kShared || p.seqlens[tok] >= p.shared_len);
+    const int lim = valid ? ((MODE != kTree && MODE != kShared && p.causal) ? min(Lk - 1, diag + tok) : Lk - 1) : -1;
     uint64_t mword = 0;
     if (MODE == kTree && valid) mword = p.tree_mask[q_begin + tok];
     // first key index at which this row needs masking
@@ -416,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
+    for (int j = 0; j < (wg == 1 && !two ? 0 : ntiles); ++j) {
       // warp-uniform: the TMEM loads below are warp-collective
       if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[wg], j & 1))) {
         ok = false;
@@ -690,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t orr[32];
       sm100::tmem_ld32(t_lane + col_o(wg) + c * 32, orr);
       sm100::tmem_wait_ld();
-      if (valid && done && p.nsplit > 1) {
+      if (valid && done && (MODE == kShared || p.nsplit > 1)) {
         const int64_t slot =
             (static_cast<int64_t>(q_begin + tok) * p.num_heads + g * group + hh) * p.nsplit + split;
         float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * kHeadDim + c * 32);
@@ -840,7 +866,7 @@ constexpr int kSmemBytes = kSmemData + 1024 + static_cast<int>(sizeof(Barriers))
 // raised. File scope (internal linkage), so every copy of the library keeps
 // its own flags.
 static std::mutex g_attr_mu;
-static bool g_attr_done[3][64];
+static bool g_attr_done[4][64];
 
 template <int MODE>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p,
@@ -879,7 +905,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return cuda_fail(e, "attn_tc_kernel launch");
-  if (p.nsplit > 1) {
+  if (MODE != kShared && p.nsplit > 1) {
     const int per_seq = max_tokens * p.num_heads;
     tree_combine_kernel<<<dim3((per_seq + 3) / 4, num_seqs), 128, 0, stream>>>(p);
     e = cudaGetLastError();
@@ -984,6 +1010,51 @@ static size_t tree_ws_bytes(int num_seqs, int64_t total_q, int num_heads, int ns
     bytes += o_bytes + n * sizeof(float2);
   }
   return bytes;
+}
+
+// Shared mode: the split of the prefix whose (row block, KV head, split) CTAs
+// take the fewest rounds of tiles. A round is one CTA per SM; every CTA pays
+// about three tiles' time to start and to write its partials.
+void shared_split(int batch, int num_heads, int num_kv_heads, int shared_len, int* nsplit,
+                  int* split_tiles) {
+  const int tpt = tc::kBM / (num_heads / num_kv_heads);
+  const int64_t items = static_cast<int64_t>((batch + 2 * tpt - 1) / (2 * tpt)) * num_kv_heads;
+  const int tiles = shared_len / tc::kBN;
+  const int sms = sm_count();
+  int64_t best = -1;
+  for (int ns = 1; ns <= std::min(tiles, 64); ++ns) {
+    const int per = (tiles + ns - 1) / ns;
+    const int live = (tiles + per - 1) / per;  // splits that have a tile
+    const int64_t cost = (items * live + sms - 1) / sms * (per + 3);
+    if (best < 0 || cost < best) {
+      best = cost;
+      *nsplit = live;
+      *split_tiles = per;
+    }
+  }
+}
+
+int launch_shared_prefix(const SharedPrefix& a, cudaStream_t stream) {
+  tc::Params p = tc_params(nullptr, 0, 0, a.num_heads, a.num_kv_heads, 1.f, a.batch, a.status);
+  p.scale_log2 = a.scale_log2;
+  CUtensorMap qm, km, vm;
+  int rc = tc::make_q_map(&qm, a.q, a.batch, a.num_heads, a.q_stride_tok, a.q_stride_head, p.group,
+                          p.tpt);
+  if (rc) return rc;
+  rc = tc::make_kv_map(&km, a.k, true, 0, a.num_blocks, a.block_size, a.num_kv_heads, 0, 0);
+  if (rc) return rc;
+  rc = tc::make_kv_map(&vm, a.v, true, 0, a.num_blocks, a.block_size, a.num_kv_heads, 0, 0);
+  if (rc) return rc;
+  p.block_table = a.block_table;
+  p.num_blocks = a.num_blocks;
+  p.block_size = a.block_size;
+  p.seqlens = a.seqlens;
+  p.shared_len = a.shared_len;
+  p.nsplit = a.nsplit;
+  p.split_tiles = a.split_tiles;
+  p.ws_o = a.ws_o;
+  p.ws_ml = a.ws_ml;
+  return tc::launch<tc::kShared>(qm, km, vm, p, 1, a.batch, stream);
 }
 
 }  // namespace nvattn

@@ -42,6 +42,9 @@ constexpr int kStageBytes = 4 * kHalfBytes;    // K lo/hi + V lo/hi (32 KB)
 constexpr int kMinSplitTiles = NVATTN_DEC_MIN_SPLIT_TILES;
 constexpr int kSplitCtasPerSm = NVATTN_DEC_SPLIT_CTAS_PER_SM;
 
+// kSuffix: the row's keys behind a shared prefix, as fp32 partials
+// (shared_prefix.cu).
+template <bool kSuffix>
 __global__ void __launch_bounds__(kDecThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const DecodeParams p) {
@@ -53,12 +56,14 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     if (split == 0 && threadIdx.x == 0) set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
     ctx = p.max_blocks * p.block_size;
   }
-  const int tok_begin = split * p.split_tiles * kTile;
-  const int tok_end = min(ctx, tok_begin + p.split_tiles * kTile);
+  const KeyRange own = kSuffix ? own_keys(p, ctx) : KeyRange{0, p.split_tiles * kTile};
+  const int tok_begin = own.begin + split * own.split;
+  const int tok_end = min(ctx, tok_begin + own.split);
   if (tok_end <= tok_begin) {
+    if (kSuffix) join_prefix_grid();
     // Whole CTA idle (uniform exit). Without a combine pass the empty
     // sequence's output rows still have to be written (as zeros).
-    if (p.nsplit == 1 && split == 0) {
+    if (!kSuffix && p.nsplit == 1 && split == 0) {
       for (int e = threadIdx.x; e < p.group * kHeadDim; e += blockDim.x) {
         const int h = g * p.group + e / kHeadDim;
         p.out[static_cast<int64_t>(b) * p.o_stride_tok + static_cast<int64_t>(h) * p.o_stride_head +
@@ -304,7 +309,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       acc += obuf[(w * kMaxGroup + r) * kOPad + d] * f;
     }
     const int h = h0 + r;
-    if (p.nsplit == 1) {
+    if (!kSuffix && p.nsplit == 1) {
       const float v = (L > 0.f) ? acc / L : 0.f;
       p.out[static_cast<int64_t>(b) * p.o_stride_tok + static_cast<int64_t>(h) * p.o_stride_head +
             d] = __float2bfloat16_rn(v);
@@ -314,6 +319,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       if (d == 0) p.ws_ml[slot] = make_float2(mmax, L);
     }
   }
+  if (kSuffix) join_prefix_grid();
 }
 
 // Merges the split-K partials of one (sequence, query head) per warp-group.
@@ -406,15 +412,21 @@ static int launch_decode_combine(const DecodeParams& p, int batch, cudaStream_t 
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "decode_combine launch");
 }
 
-static int set_smem_attr(const void* fn, int bytes) {
+constexpr int kDecSmem = kDecStages * kStageBytes + 1024 + 2 * kDecStages * 8 +
+                         kDecConsumerWarps * kMaxGroup * 2 * 4;
+
+template <bool kSuffix>
+static int set_smem_attr() {
   // Per device: the attribute must be set once in every context that launches.
   static std::mutex mu;
   static int done[64] = {0};
+  constexpr int bytes = kDecSmem;
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(mu);
   if (dev < 64 && done[dev] >= bytes) return NVATTN_OK;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<kSuffix>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
   if (dev < 64) done[dev] = bytes;
   return NVATTN_OK;
@@ -431,6 +443,29 @@ int make_cache_map(CUtensorMap* map, const void* cache, int num_blocks, int bloc
       static_cast<uint64_t>(block_size) * num_kv_heads * kHeadDim * 2};
   const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kTile), 1};
   return make_tensor_map(map, cache, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int launch_decode_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache, int batch,
+                         bool after_prefix, cudaStream_t stream) {
+  CUtensorMap kmap, vmap;
+  int rc = make_cache_map(&kmap, k_cache, p.num_blocks, p.block_size, p.num_kv_heads);
+  if (rc) return rc;
+  rc = make_cache_map(&vmap, v_cache, p.num_blocks, p.block_size, p.num_kv_heads);
+  if (rc) return rc;
+  rc = set_smem_attr<true>();
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.nsplit, p.num_kv_heads, batch);
+  cfg.blockDim = dim3(kDecThreads);
+  cfg.dynamicSmemBytes = kDecSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_prefix ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<true>, kmap, vmap, p);
+  return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode (own keys) launch");
 }
 
 // A negative batch is an error; the caller handles batch == 0 before.
@@ -530,14 +565,12 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
   p.status = status;
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
 
-  const int smem = kDecStages * kStageBytes + 1024 + 2 * kDecStages * 8 +
-                   kDecConsumerWarps * kMaxGroup * 2 * 4;
-  rc = set_smem_attr(reinterpret_cast<const void*>(paged_decode_kernel), smem);
+  rc = set_smem_attr<false>();
   if (rc) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (batch > 65535) return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode: batch > 65535");
   dim3 grid(nsplit, num_kv_heads, batch);
-  paged_decode_kernel<<<grid, kDecThreads, smem, s>>>(kmap, vmap, p);
+  paged_decode_kernel<false><<<grid, kDecThreads, kDecSmem, s>>>(kmap, vmap, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_decode launch");
   return nsplit > 1 ? launch_decode_combine(p, batch, s) : NVATTN_OK;

@@ -32,6 +32,27 @@ struct DecodeParams {
 
 __device__ __forceinline__ float neg_inf() { return -INFINITY; }
 
+// The keys of a row that the decode kernels own beside a shared prefix of
+// p.key_begin keys: from the prefix's end on, p.split_tiles tiles a split. A
+// row shorter than the prefix takes no part in the prefix: its keys are all its
+// own, in splits long enough for the grid. (key_begin 0: all keys.)
+struct KeyRange {
+  int begin, split;  // first key, keys a split
+};
+__device__ __forceinline__ KeyRange own_keys(const DecodeParams& p, int ctx) {
+  if (ctx >= p.key_begin) return {p.key_begin, p.split_tiles * kTile};
+  const int tiles = (max(ctx, 0) + kTile - 1) / kTile;
+  return {0, max(p.split_tiles, (tiles + p.nsplit - 1) / p.nsplit) * kTile};
+}
+
+// One CTA of a kernel launched beside the prefix's kernel (its programmatic
+// dependent) ends only after that grid has completed, so whatever waits for
+// this kernel has the prefix's partials too.
+__device__ __forceinline__ void join_prefix_grid() {
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Split size for a batch over tables of max_blocks (see decode.cu).
 void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size, int* nsplit,
                   int* split_tiles);
@@ -46,6 +67,15 @@ int check_decode_args(const char* who, const void* q, int64_t q_stride_tok, int6
                       int64_t block_table_stride, int32_t max_blocks_per_seq, int32_t num_blocks,
                       int32_t block_size, int32_t batch, int32_t num_heads, int32_t num_kv_heads,
                       int32_t head_dim);
+// The suffix kernels over p's own keys; after_prefix: as programmatic
+// dependents of the prefix's kernel, launched just before on `stream`.
+int launch_decode_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache, int batch,
+                         bool after_prefix, cudaStream_t stream);
+int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
+                             const uint8_t* k_scale, const uint8_t* v_scale, int batch,
+                             bool after_prefix, cudaStream_t stream);
+// Checks an fp8 cache's scale pointers.
+int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale);
 // Merges partials of up to two key ranges into p.out: `first` (nfirst of them, all
 // live in a row with keys; p.key_begin keys together) and p's own nsplit ones.
 int launch_merge_partials(const DecodeParams& p, const float* first_o, const float2* first_ml,

@@ -138,10 +138,12 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     if (split == 0 && threadIdx.x == 0) set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
     ctx = p.max_blocks * p.block_size;
   }
-  const int tok_begin = (kSuffix ? p.key_begin : 0) + split * p.split_tiles * kTile;
-  const int tok_end = min(ctx, tok_begin + p.split_tiles * kTile);
+  const KeyRange own = kSuffix ? own_keys(p, ctx) : KeyRange{0, p.split_tiles * kTile};
+  const int tok_begin = own.begin + split * own.split;
+  const int tok_end = min(ctx, tok_begin + own.split);
   if (tok_end <= tok_begin) {
-    if (!kSuffix && p.nsplit == 1) {  // no merge runs: the empty row's zeros
+    if (kSuffix) join_prefix_grid();
+    if (!kSuffix && p.nsplit == 1 && split == 0) {  // no merge runs: the empty row's zeros
       for (int e = threadIdx.x; e < p.group * kHeadDim; e += blockDim.x)
         p.out[static_cast<int64_t>(b) * p.o_stride_tok +
               static_cast<int64_t>(g * p.group + e / kHeadDim) * p.o_stride_head + e % kHeadDim] =
@@ -397,6 +399,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       if (d == 0) p.ws_ml[slot] = make_float2(mmax, L);
     }
   }
+  if (kSuffix) join_prefix_grid();
 }
 
 // Merges the partials of one (sequence, query head) per warp: lane i owns dims
@@ -413,10 +416,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   if (row >= rows) return;
   const int b = row / p.num_heads, h = row - b * p.num_heads;
   const int ctx = min(p.seqlens[b], p.max_blocks * p.block_size);
-  const int split_tokens = p.split_tiles * kTile;
-  const int own = max(ctx - p.key_begin, 0);
-  const int nf = ctx > 0 ? nfirst : 0;
-  const int n = nf + min(p.nsplit, (own + split_tokens - 1) / split_tokens);
+  const KeyRange own = own_keys(p, ctx);
+  const int nf = own.begin > 0 ? nfirst : 0;
+  const int n = nf + min(p.nsplit, (max(ctx - own.begin, 0) + own.split - 1) / own.split);
   // partials 0..nf-1 are the first range's, nf..n-1 the own ones
   const int64_t fbase = static_cast<int64_t>(row) * nfirst;
   const int64_t obase = static_cast<int64_t>(row) * p.nsplit;
@@ -506,9 +508,9 @@ static int raise_smem8() {
 }
 
 template <bool kSuffix>
-int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const void* v_cache,
-                      const uint8_t* k_scale, const uint8_t* v_scale, int batch,
-                      cudaStream_t stream) {
+static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const void* v_cache,
+                             const uint8_t* k_scale, const uint8_t* v_scale, int batch,
+                             bool after_prefix, cudaStream_t stream) {
   CUtensorMap kmap, vmap;
   int rc = make_cache8_map(&kmap, k_cache, p.num_blocks, p.block_size, p.num_kv_heads);
   if (rc) return rc;
@@ -516,11 +518,26 @@ int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const void* v_
   if (rc) return rc;
   rc = raise_smem8<kSuffix>();
   if (rc) return rc;
-  paged_decode_fp8_kernel<kSuffix>
-      <<<dim3(p.nsplit, p.num_kv_heads, batch), kDecThreads, kSmem8, stream>>>(
-          kmap, vmap, k_scale, v_scale, p);
-  const cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.nsplit, p.num_kv_heads, batch);
+  cfg.blockDim = dim3(kDecThreads);
+  cfg.dynamicSmemBytes = kSmem8;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_prefix ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_fp8_kernel<kSuffix>, kmap, vmap,
+                                           k_scale, v_scale, p);
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode_fp8 launch");
+}
+
+int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
+                             const uint8_t* k_scale, const uint8_t* v_scale, int batch,
+                             bool after_prefix, cudaStream_t stream) {
+  return launch_decode_fp8<true>(p, k_cache, v_cache, k_scale, v_scale, batch, after_prefix,
+                                 stream);
 }
 
 int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale) {
@@ -580,7 +597,7 @@ extern "C" int nvattn_paged_decode_fp8(
     return fail(NVATTN_ERR_INVALID, "paged_decode_fp8: workspace must be 256-byte aligned");
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  rc = launch_decode_fp8<false>(p, k_cache, v_cache, k_scale, v_scale, batch, s);
+  rc = launch_decode_fp8<false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s);
   if (rc || p.nsplit == 1) return rc;
   return launch_merge_partials(p, nullptr, nullptr, 0, batch, s);
 }

@@ -21,7 +21,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace nvattn {
 
@@ -155,7 +155,8 @@ constexpr int kLoadRows = 4;
 
 // CTA: kLoadRows * kLoadThreads / 8 consecutive (key, KV head) rows of the
 // dense output. The sequence of a CTA's first key is found by bisection of
-// cu_seqlens_k, the others by walking on from it.
+// cu_seqlens_k, the others by walking on from it (cu_k null: one sequence of
+// all rows).
 __global__ void __launch_bounds__(kLoadThreads)
     load_kvcache_fp8_kernel(const uint8_t* __restrict__ k_cache,
                             const uint8_t* __restrict__ v_cache,
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(kLoadThreads)
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kLoadRows * kStep;
   // last sequence whose start is <= the CTA's first key
   int seq = 0;
-  {
+  if (cu_k != nullptr) {
     const int64_t key0 = first / num_kv_heads;
     int hi = num_seqs;
     while (hi - seq > 1) {
@@ -194,8 +195,11 @@ __global__ void __launch_bounds__(kLoadThreads)
     if (row >= num_rows) continue;
     const int64_t key = row / num_kv_heads;
     const int g = static_cast<int>(row - key * num_kv_heads);
-    while (seq < num_seqs && key >= __ldg(cu_k + seq + 1)) ++seq;
-    const int64_t pos = seq < num_seqs ? key - __ldg(cu_k + seq) : -1;
+    int64_t pos = key;
+    if (cu_k != nullptr) {
+      while (seq < num_seqs && key >= __ldg(cu_k + seq + 1)) ++seq;
+      pos = seq < num_seqs ? key - __ldg(cu_k + seq) : -1;
+    }
     if (pos < 0) {  // behind the last sequence, or before the first
       if (zero_rest) out_row[u] = row;
       continue;

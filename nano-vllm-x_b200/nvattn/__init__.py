@@ -12,15 +12,15 @@ from . import ops, tree, parallel, decode_meta
 from .decode_meta import DecodeMetadata
 from .ops import (flash_attn_varlen_func, flash_attn_with_kvcache, kv_move, load_kvcache_fp8,
                   paged_decode, paged_decode_fp8, qk_norm_rope_store, sample, sample_merge,
-                  sample_shard, store_kvcache, store_kvcache_fp8, tree_attention, varlen_prefill,
-                  verify_draft)
+                  sample_shard, shared_prefix_decode, store_kvcache, store_kvcache_fp8,
+                  tree_attention, varlen_prefill, verify_draft)
 
 __all__ = [
     "Attention", "Context", "get_context", "set_context", "reset_context", "ops", "tree",
     "parallel", "store_kvcache", "varlen_prefill", "paged_decode", "tree_attention", "kv_move",
     "flash_attn_varlen_func", "flash_attn_with_kvcache", "qk_norm_rope_store", "sample",
     "sample_shard", "sample_merge", "store_kvcache_fp8", "load_kvcache_fp8", "paged_decode_fp8",
-    "verify_draft", "DecodeMetadata", "decode_meta", "install",
+    "shared_prefix_decode", "verify_draft", "DecodeMetadata", "decode_meta", "install",
 ]
 
 

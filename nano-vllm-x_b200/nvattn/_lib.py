@@ -65,6 +65,12 @@ SIGNATURES: dict[str, tuple] = {
                                         _I32P, _I32P, c_int64, c_int32, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int32, c_float, _P, c_size_t,
                                         _I32P, _P]),
+    "nvattn_shared_prefix_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32,
+                                                        c_int32, c_int32]),
+    "nvattn_shared_prefix_decode": (c_int, [_P, c_int64, c_int64, _P, _P, _P, _P, _P, c_int64,
+                                            c_int64, _I32P, _I32P, c_int64, c_int32, c_int32,
+                                            c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                            c_float, _P, c_size_t, _I32P, _P]),
     "nvattn_tree_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int64, c_int32, c_int32,
                                                c_int32, c_int32]),
     "nvattn_tree_verify": (c_int, [_P, c_int64, c_int64,

@@ -20,6 +20,8 @@ on a machine without the CUDA library these functions raise.
     store_kvcache_fp8,       new: the cache in 8-bit floating point — scatter
     load_kvcache_fp8,        with quantisation, read back as dense bf16 rows,
     paged_decode_fp8         decode attention over it
+    shared_prefix_decode     new: decode attention with the keys that all
+                             sequences share read once for the batch
     verify_draft             new: which drafted tokens stand against the
                              target's probabilities, and the token after them
 
@@ -47,6 +49,8 @@ __all__ = [
     "store_kvcache_fp8",
     "load_kvcache_fp8",
     "paged_decode_fp8",
+    "shared_prefix_decode",
+    "shared_prefix_workspace_bytes",
     "qk_norm_rope_store",
     "sample",
     "sample_shard",
@@ -487,6 +491,62 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                   out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),
                   block_table.data_ptr(), block_table.stride(0), max_blocks, num_blocks,
                   block_size, batch, num_heads, num_kv_heads, head_dim,
+                  head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
+                  ws_bytes, _status_ptr(dev), _stream(dev))
+    return out
+
+
+# ---------------------------------------------------------------- shared prefix
+
+def shared_prefix_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, max_blocks: int,
+                                  block_size: int, shared_len: int, fp8: bool = False) -> int:
+    return int(_lib.load().nvattn_shared_prefix_workspace_bytes(
+        batch, num_heads, num_kv_heads, max_blocks, block_size, shared_len, 1 if fp8 else 0))
+
+
+def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         cache_seqlens: torch.Tensor, block_table: torch.Tensor, shared_len: int,
+                         softmax_scale: float | None = None, k_scale: torch.Tensor | None = None,
+                         v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_decode`` for a batch whose sequences share their first ``shared_len`` keys.
+
+    The shared pages are the first shared_len / block_size entries of row 0 of
+    block_table, read once for the whole batch; keys behind them come through
+    each sequence's own row. cache_seqlens counts all keys; a row with fewer
+    than shared_len (0: padding, zeros) is attended over its own row alone.
+    shared_len must be whole blocks, block_size a multiple of 128. With
+    k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
+    ``workspace``: uint8, ``shared_prefix_workspace_bytes`` of the same sizes.
+    """
+    dev = _require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out,
+                        workspace)
+    fp8 = k_scale is not None
+    if fp8 != (v_scale is not None):
+        raise ValueError("give both k_scale and v_scale, or neither")
+    if fp8:
+        num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale,
+                                                                 v_scale)
+    else:
+        _check_bf16(k_cache, v_cache)
+        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+            raise ValueError("caches must be (num_blocks, block_size, kv_heads, d)")
+        if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous")
+        num_blocks, block_size, num_kv_heads = k_cache.shape[:3]
+    batch, num_heads, head_dim, out = _check_decode(q, out, cache_seqlens, block_table,
+                                                    num_kv_heads, k_cache.shape[3])
+    shared_len, max_blocks = int(shared_len), block_table.shape[1]
+    with _device(dev):
+        ws_ptr, ws_bytes = _workspace(
+            shared_prefix_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size,
+                                          shared_len, fp8), workspace, dev)
+        _lib.call("nvattn_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1),
+                  k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if fp8 else None,
+                  v_scale.data_ptr() if fp8 else None, out.data_ptr(), out.stride(0),
+                  out.stride(1), cache_seqlens.data_ptr(), block_table.data_ptr(),
+                  block_table.stride(0), max_blocks, num_blocks, block_size, shared_len, batch,
+                  num_heads, num_kv_heads, head_dim,
                   head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
                   ws_bytes, _status_ptr(dev), _stream(dev))
     return out
