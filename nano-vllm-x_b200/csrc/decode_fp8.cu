@@ -1,6 +1,5 @@
 // Paged split-K decode attention over the fp8 cache (layout and rounding in
-// kvcache_fp8.cu): the split, the grid and the roles of decode.cu, half the
-// bytes.
+// kvcache_fp8.cu): the split and the grid of decode.cu, half the bytes.
 //
 //   o = sum_j softmax_j(c * 2^kk_j * q.k8_j) * 2^kv_j * v8_j
 //
@@ -15,11 +14,13 @@
 // brought in by a power of two a row, so only elements below 2^-14 of the
 // row's largest lose bits (2^-25 of it).
 //
-// HBM-bound: 258 bytes a (key, KV head) against 4 * 128 * group flops. The
-// cost to hide is the conversion, 2 instructions for 4 elements and one byte
-// permute for V: a warp owns whole 64-key tiles (the four warps of a CTA take
-// turns), so the row maxima, the barrier waits and the rescale are paid once
-// for 64 keys.
+// HBM-bound: 258 bytes a (key, KV head) against 4 * 128 * group flops. What is
+// left to hide is the arithmetic around the products, so the keys are the M
+// rows of the MMAs and the query heads the 8 columns (S^T = K Q^T, O^T =
+// V^T W^T): with up to 8 heads a group no MMA row and no softmax lane is
+// padding, and the conversions (2 a 4-byte word, plus one byte permute for V)
+// serve all heads. A warp owns whole 64-key tiles, the warps of a CTA taking
+// turns, so maxima, barrier waits and rescales are paid once for 64 keys.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -30,12 +31,19 @@
 namespace nvattn {
 
 constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
-constexpr int kStages8 = 6;                   // ring depth
 constexpr int kStageBytes8 = 2 * kTile8;      // K and V
 constexpr int kScaleBytes8 = 2 * kTile;       // their exponent bytes
-constexpr int kSmem8 = kStages8 * (kStageBytes8 + kScaleBytes8) + 1024 + 2 * kStages8 * 8 +
-                       kDecConsumerWarps * kMaxGroup * 2 * 4;
-static_assert(kDecConsumerWarps * kMaxGroup * kOPad * 4 <= kStages8 * kStageBytes8,
+
+// Consumer warps of a CTA for NB blocks of 8 query heads (registers a thread
+// grow with NB; two CTAs an SM either way). Each has one stage of the ring:
+// tile i goes to warp and stage i % warps, so a warp meets its stage's phases
+// one by one (a parity wait cannot tell phase n from n + 2, and copies may
+// land out of order).
+constexpr int dec8_warps(int NB) { return NB == 1 ? 6 : 4; }
+constexpr int dec8_smem(int NB) {
+  return dec8_warps(NB) * (kStageBytes8 + kScaleBytes8 + 2 * 8 + 8 * NB * 8) + 1024;
+}
+static_assert(8 * kOPad * 4 <= kStageBytes8 && 16 * kOPad * 4 <= kStageBytes8,
               "the merge buffer reuses the ring");
 
 // 1-D bulk copy into shared memory, completion on an mbarrier (16-byte
@@ -80,56 +88,57 @@ __device__ __forceinline__ float exp_byte_log2(uint32_t byte) {
   return __uint_as_float(0x4B000000u | byte) - (8388608.f + 127.f);
 }
 
-// f16 A fragments of this thread's two query rows (rowa, rowb of the group)
-// and the exact power of two they were divided by. A 16-dim step takes dims
-// 4q..4q+3 of quad lane q (dims may be summed in any order as long as K's
-// fragments agree: one 4-byte word of an e4m3 row holds them).
-__device__ __forceinline__ void load_q8(const DecodeParams& p, int b, int h0, int rowa, int rowb,
-                                        int quad, uint32_t qa[8][4], float* back_a,
-                                        float* back_b) {
-  const __nv_bfloat16* qb = p.q + static_cast<int64_t>(b) * p.q_stride_tok;
-  const uint32_t* row[2] = {
-      reinterpret_cast<const uint32_t*>(qb + static_cast<int64_t>(h0 + rowa) * p.q_stride_head),
-      reinterpret_cast<const uint32_t*>(qb + static_cast<int64_t>(h0 + rowb) * p.q_stride_head)};
-  const bool live[2] = {rowa < p.group, rowb < p.group};
-  float* back[2] = {back_a, back_b};
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    uint32_t w[16];
-    float mx = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      w[2 * kk] = live[r] ? row[r][kk * 8 + quad * 2] : 0u;
-      w[2 * kk + 1] = live[r] ? row[r][kk * 8 + quad * 2 + 1] : 0u;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)),
-                           fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // exponent of the largest element, kept where both 2^e and 2^-e are normal
-    const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 1), 253);
-    const float down = __int_as_float((254 - e) << 23);
-    *back[r] = __int_as_float(e << 23);
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        qa[kk][2 * i + r] = pack_f16x2(__uint_as_float(w[2 * kk + i] << 16) * down,
-                                       __uint_as_float(w[2 * kk + i] & 0xffff0000u) * down);
-    }
-  }
+// Transposes an 8 x 8 matrix of 16-bit elements held as one fragment register.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
-// kSuffix: the keys from p.key_begin on, as fp32 partials for the merge with
-// the keys before (shared_prefix.cu).
-template <bool kSuffix>
-__global__ void __launch_bounds__(kDecThreads, 2)
+// B fragments of query head `h` (column lane / 4): a 16-dim step takes dims
+// 4q..4q+3 of quad lane q (dims may be summed in any order as long as K's
+// fragments agree: one 4-byte word of an e4m3 row holds them). Returns the
+// exact power of two the row was divided by.
+__device__ __forceinline__ float load_q8(const __nv_bfloat16* row, bool live, int quad,
+                                         uint32_t qb[8][2]) {
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(row);
+  uint32_t w[16];
+  float mx = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    w[2 * kk] = live ? src[kk * 8 + quad * 2] : 0u;
+    w[2 * kk + 1] = live ? src[kk * 8 + quad * 2 + 1] : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)),
+                         fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  // exponent of the largest element, kept where both 2^e and 2^-e are normal
+  const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23), 1), 253);
+  const float down = __int_as_float((254 - e) << 23);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      qb[kk][i] = pack_f16x2(__uint_as_float(w[2 * kk + i] << 16) * down,
+                             __uint_as_float(w[2 * kk + i] & 0xffff0000u) * down);
+  }
+  return __int_as_float(e << 23);
+}
+
+// NB: blocks of 8 query heads (group <= 8 * NB). kSuffix: the keys from
+// p.key_begin on, as fp32 partials for the merge with the keys before
+// (shared_prefix.cu).
+template <int NB, bool kSuffix>
+__global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
     paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap,
                             const uint8_t* __restrict__ k_scale,
                             const uint8_t* __restrict__ v_scale, const DecodeParams p) {
+  constexpr int kWarps = dec8_warps(NB);
+  constexpr int kStages8 = kWarps;
   const int split = blockIdx.x;
   const int g = blockIdx.y;
   const int b = blockIdx.z;
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   uint8_t* scales = smem + kStages8 * kStageBytes8;
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + kStages8 * kScaleBytes8);
   uint64_t* empty = full + kStages8;
-  float* ml_smem = reinterpret_cast<float*>(empty + kStages8);  // [4][16][2]
+  float2* ml_smem = reinterpret_cast<float2*>(empty + kStages8);  // [warp][8 * NB heads]
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -173,7 +182,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   }
   __syncthreads();
 
-  if (warp == kDecConsumerWarps) {
+  if (warp == kWarps) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       prefetch_tensor_map(&kmap);
@@ -211,25 +220,42 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   }
 
   // -------------------------------------------------------------- consumers
-  const int quad = lane & 3;   // column pair inside an 8-wide MMA tile
-  const int rowa = lane >> 2;  // accumulator rows rowa and rowa + 8
-  const int rowb = rowa + 8;
+  const int quad = lane & 3;  // this lane's head columns 2*quad, 2*quad + 1 of each block
+  const int sub = lane >> 2;  // its key (or dim pair) inside 8
   const int h0 = g * p.group;
 
-  uint32_t qa[8][4];
-  float scale_a, scale_b;
-  load_q8(p, b, h0, rowa, rowb, quad, qa, &scale_a, &scale_b);
-  scale_a *= p.scale_log2;
-  scale_b *= p.scale_log2;
-
-  // o[2c + e] holds dims 16c + 4*quad + {0, 2} + e of rows rowa, rowb
-  float o[16][4];
+  uint32_t qb[NB][8][2];
+  float scale[NB][2];  // of head columns 2*quad, 2*quad + 1
 #pragma unroll
-  for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m_a = neg_inf(), m_b = neg_inf(), l_a = 0.f, l_b = 0.f;
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = nb * 8 + sub;
+    const float back =
+        load_q8(p.q + static_cast<int64_t>(b) * p.q_stride_tok +
+                    static_cast<int64_t>(h0 + min(r, p.group - 1)) * p.q_stride_head,
+                r < p.group, quad, qb[nb]);
+    scale[nb][0] = __shfl_sync(0xffffffffu, back, quad * 8) * p.scale_log2;
+    scale[nb][1] = __shfl_sync(0xffffffffu, back, quad * 8 + 4) * p.scale_log2;
+  }
+
+  // o[c][nb][2e + j]: dim 16c + 2*sub + e of head column 2*quad + j
+  float o[8][NB][4];
+  float m[NB][2], l[NB][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c][nb][0] = o[c][nb][1] = o[c][nb][2] = o[c][nb][3] = 0.f;
+    m[nb][0] = m[nb][1] = neg_inf();
+    l[nb][0] = l[nb][1] = 0.f;
+  }
+
+  // ldmatrix addresses: row lane % 16 of a 16-key step, chunk pair member
+  // lane / 16 (128-byte rows, 128-byte swizzle)
+  uint32_t off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) off[i] = swz128(lane & 15, 2 * i + (lane >> 4));
 
   bool timed_out = false;
-  for (int it = warp; it < ntiles; it += kDecConsumerWarps) {
+  for (int it = warp; it < ntiles; it += kWarps) {
     const int stage = it % kStages8;
     if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (it / kStages8) & 1))) {
       timed_out = true;
@@ -240,104 +266,131 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     const uint8_t* ss = scales + stage * kScaleBytes8;
     const uint32_t kbase = smem_u32(st);
     const uint32_t vbase = kbase + kTile8;
-    if (nvalid < kTile) {
-      // Keys past the end hold stale bytes (maybe NaN): zero their V rows so
-      // that 0 * NaN never reaches the sum. Only a range's last tile has
-      // them, so no later copy lands in this stage.
-      for (int e = lane; e < (kTile - nvalid) * 8; e += 32)
-        *reinterpret_cast<int4*>(st + kTile8 + nvalid * 128 + e * 16) = make_int4(0, 0, 0, 0);
-      __syncwarp();
+    // ---- S^T = K Q^T: 4 steps of 16 keys, 8 of 16 dims
+    float s[4][NB][4];  // [mt][nb][2e + j]: key 16mt + 8e + sub, head column 2*quad + j
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[mt][nb][0] = s[mt][nb][1] = s[mt][nb][2] = s[mt][nb][3] = 0.f;
     }
-    // ---- S = Q K^T: 8 tiles of 8 keys, 8 steps of 16 dims
-    float s[8][4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      const int row = n * 8 + (lane & 7);
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[4];  // this lane's 4 bytes of steps 4*half .. 4*half + 3
-        ldmatrix_x4(kbase + swz128(row, half * 4 + (lane >> 3)), w[0], w[1], w[2], w[3]);
+      for (int mt = 0; mt < 4; ++mt) {
+        uint32_t w[4];  // this lane's 4 bytes: keys 0-7 and 8-15 of steps 2i, 2i + 1
+        ldmatrix_x4(kbase + mt * 2048 + off[i], w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mma_f16_16816(s[n], qa[half * 4 + i], e4m3x2_to_f16x2(w[i]),
-                        e4m3x2_to_f16x2(w[i] >> 16));
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a[4] = {e4m3x2_to_f16x2(w[2 * j]), e4m3x2_to_f16x2(w[2 * j + 1]),
+                                 e4m3x2_to_f16x2(w[2 * j] >> 16),
+                                 e4m3x2_to_f16x2(w[2 * j + 1] >> 16)};
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            mma_f16_16816(s[mt][nb], a, qb[nb][2 * i + j][0], qb[nb][2 * i + j][1]);
+        }
       }
     }
     // ---- exponents, mask, online softmax
-    float mx_a = neg_inf(), mx_b = neg_inf();
-    float ve[8][2];
+    float ve[4][2];  // exponents of V, [mt][e]
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const uint32_t kb = *reinterpret_cast<const uint16_t*>(ss + n * 8 + quad * 2);
-      const uint32_t vb = *reinterpret_cast<const uint16_t*>(ss + kTile + n * 8 + quad * 2);
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int t = mt * 16 + e * 8 + sub;
+        const float kf = exp_byte_scale(ss[t]);
+        ve[mt][e] = exp_byte_log2(ss[kTile + t]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          s[mt][nb][2 * e] *= scale[nb][0] * kf;
+          s[mt][nb][2 * e + 1] *= scale[nb][1] * kf;
+        }
+      }
+    }
+    if (nvalid < kTile) {
+      // Keys past the end hold stale bytes (maybe NaN): their scores are
+      // masked, and their V rows zeroed so that 0 * NaN never reaches the sum.
+      // Only a range's last tile has them, so no later copy lands in this
+      // stage.
+      for (int e = lane; e < (kTile - nvalid) * 8; e += 32)
+        *reinterpret_cast<int4*>(st + kTile8 + nvalid * 128 + e * 16) = make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (mt * 16 + e * 8 + sub >= nvalid) {
+            ve[mt][e] = 0.f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) s[mt][nb][2 * e] = s[mt][nb][2 * e + 1] = neg_inf();
+          }
+        }
+      }
+      __syncwarp();
+    }
+    float mn[NB][2];
+    bool grew = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const bool ok = n * 8 + quad * 2 + j < nvalid;
-        const float kf = exp_byte_scale((kb >> (8 * j)) & 0xffu);
-        ve[n][j] = ok ? exp_byte_log2((vb >> (8 * j)) & 0xffu) : 0.f;
-        s[n][j] = ok ? s[n][j] * (scale_a * kf) : neg_inf();
-        s[n][2 + j] = ok ? s[n][2 + j] * (scale_b * kf) : neg_inf();
-        mx_a = fmaxf(mx_a, s[n][j] + ve[n][j]);
-        mx_b = fmaxf(mx_b, s[n][2 + j] + ve[n][j]);
+        float mx = neg_inf();
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+          mx = fmax3(mx, s[mt][nb][j] + ve[mt][0], s[mt][nb][2 + j] + ve[mt][1]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mn[nb][j] = fmaxf(m[nb][j], mx);
+        grew |= mn[nb][j] > m[nb][j];
       }
     }
-    mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
-    mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
-    mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
-    mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
-    const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
-    if (__any_sync(0xffffffffu, mn_a > m_a || mn_b > m_b)) {
-      // l in two half steps: with V rows of very different magnitudes the
-      // factor alone can leave fp32's range while its product with l does not
-      const float h_a = fast_exp2(0.5f * (m_a - mn_a)), h_b = fast_exp2(0.5f * (m_b - mn_b));
-      l_a = l_a * h_a * h_a;
-      l_b = l_b * h_b * h_b;
-      const float al_a = h_a * h_a, al_b = h_b * h_b;
+    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        o[j][0] *= al_a;
-        o[j][1] *= al_a;
-        o[j][2] *= al_b;
-        o[j][3] *= al_b;
-      }
-      m_a = mn_a;
-      m_b = mn_b;
-    }
-    // ---- O += W V: 4 steps of 16 keys
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t pa[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = 2 * kk + i;
-        float w[4];
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float ta = s[n][j] - m_a, tb = s[n][2 + j] - m_b;
-          l_a += fast_exp2(ta);
-          l_b += fast_exp2(tb);
-          w[j] = fast_exp2(ta + ve[n][j]);
-          w[2 + j] = fast_exp2(tb + ve[n][j]);
+          // l in two half steps: with V rows of very different magnitudes the
+          // factor alone can leave fp32's range while its product with l does not
+          const float h = fast_exp2(0.5f * (m[nb][j] - mn[nb][j]));
+          l[nb][j] = l[nb][j] * h * h;
+          const float al = h * h;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            o[c][nb][j] *= al;
+            o[c][nb][2 + j] *= al;
+          }
+          m[nb][j] = mn[nb][j];
         }
-        pa[2 * i] = pack_f16x2(w[0], w[1]);
-        pa[2 * i + 1] = pack_f16x2(w[2], w[3]);
       }
-      const int row = kk * 16 + (lane & 15);
+    }
+    // ---- O^T += V^T W^T: 4 steps of 16 keys
 #pragma unroll
-      for (int c = 0; c < 8; c += 2) {
-        // keys 2q, 2q+1 (r0, r2) and 2q+8, 2q+9 (r1, r3) of dims 2i, 2i+1 of
-        // chunks c (r0, r1) and c+1 (r2, r3), i = lane / 4
+    for (int mt = 0; mt < 4; ++mt) {
+      uint32_t wb[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float t0 = s[mt][nb][2 * e] - m[nb][0], t1 = s[mt][nb][2 * e + 1] - m[nb][1];
+          l[nb][0] += fast_exp2(t0);
+          l[nb][1] += fast_exp2(t1);
+          wb[nb][e] = transpose8x8(
+              pack_f16x2(fast_exp2(t0 + ve[mt][e]), fast_exp2(t1 + ve[mt][e])));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // keys 2q, 2q+1 of dims 2*sub, 2*sub+1: keys 0-7 and 8-15 of chunks 2i, 2i + 1
         uint32_t r[4];
-        ldmatrix_x4_trans(vbase + swz128(row, c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        ldmatrix_x4_trans(vbase + mt * 2048 + off[i], r[0], r[1], r[2], r[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0, 0x3120);  // pair the keys
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t lo = __byte_perm(r[2 * j], 0, 0x3120);  // pair the keys
+          const uint32_t hi = __byte_perm(r[2 * j + 1], 0, 0x3120);
+          const uint32_t a[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16),
+                                 e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16)};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma_f16_16816(o[2 * (c + i)], pa, e4m3x2_to_f16x2(r[2 * i]),
-                        e4m3x2_to_f16x2(r[2 * i + 1]));
-          mma_f16_16816(o[2 * (c + i) + 1], pa, e4m3x2_to_f16x2(r[2 * i] >> 16),
-                        e4m3x2_to_f16x2(r[2 * i + 1] >> 16));
+          for (int nb = 0; nb < NB; ++nb)
+            mma_f16_16816(o[2 * i + j][nb], a, wb[nb][0], wb[nb][1]);
         }
       }
     }
@@ -347,47 +400,40 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   if (timed_out && lane == 0) set_status(p.status, NVATTN_STATUS_TIMEOUT);
 
   // ---------------------------------------------------------------- merge
-  l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
-  l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
-  l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
-  l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
-
   // All consumer warps are past their last ring read: reuse the ring.
-  asm volatile("bar.sync 1, %0;" ::"r"(kDecConsumerWarps * 32));
-  float* obuf = reinterpret_cast<float*>(smem);  // [4 warps][16 rows][kOPad]
-  float* ow = obuf + warp * kMaxGroup * kOPad;
-  if (quad == 0) {
-    ml_smem[(warp * kMaxGroup + rowa) * 2 + 0] = m_a;
-    ml_smem[(warp * kMaxGroup + rowa) * 2 + 1] = l_a;
-    ml_smem[(warp * kMaxGroup + rowb) * 2 + 0] = m_b;
-    ml_smem[(warp * kMaxGroup + rowb) * 2 + 1] = l_b;
-  }
+  asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32));
+  float* obuf = reinterpret_cast<float*>(smem);  // [warp][8 * NB heads][kOPad]
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const int d = c * 16 + quad * 4;
-    *reinterpret_cast<float4*>(ow + rowa * kOPad + d) =
-        make_float4(o[2 * c][0], o[2 * c + 1][0], o[2 * c][1], o[2 * c + 1][1]);
-    *reinterpret_cast<float4*>(ow + rowb * kOPad + d) =
-        make_float4(o[2 * c][2], o[2 * c + 1][2], o[2 * c][3], o[2 * c + 1][3]);
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = warp * 8 * NB + nb * 8 + quad * 2 + j;
+      float sum = l[nb][j];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (sub == 0) ml_smem[r] = make_float2(m[nb][j], sum);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float2*>(obuf + r * kOPad + c * 16 + sub * 2) =
+            make_float2(o[c][nb][j], o[c][nb][2 + j]);
+    }
   }
-  asm volatile("bar.sync 1, %0;" ::"r"(kDecConsumerWarps * 32));
+  asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32));
 
-  const int d = threadIdx.x;  // 0..127: one head-dim column per thread
-  for (int r = 0; r < p.group; ++r) {
-    float mw[kDecConsumerWarps];
+  for (int e = threadIdx.x; e < p.group * kHeadDim; e += kWarps * 32) {
+    const int r = e / kHeadDim, d = e % kHeadDim;
     float mmax = neg_inf();
 #pragma unroll
-    for (int w = 0; w < kDecConsumerWarps; ++w) {
-      mw[w] = ml_smem[(w * kMaxGroup + r) * 2];
-      mmax = fmaxf(mmax, mw[w]);
-    }
+    for (int w = 0; w < kWarps; ++w) mmax = fmaxf(mmax, ml_smem[w * 8 * NB + r].x);
     float L = 0.f, acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecConsumerWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       // a warp without a tile keeps m = -inf, l = 0, o = 0
-      const float h = (mw[w] == neg_inf()) ? 0.f : fast_exp2(0.5f * (mw[w] - mmax));
-      L += ml_smem[(w * kMaxGroup + r) * 2 + 1] * h * h;
-      acc += obuf[(w * kMaxGroup + r) * kOPad + d] * h * h;
+      const float2 ml = ml_smem[w * 8 * NB + r];
+      const float h = (ml.x == neg_inf()) ? 0.f : fast_exp2(0.5f * (ml.x - mmax));
+      L += ml.y * h * h;
+      acc += obuf[(w * 8 * NB + r) * kOPad + d] * h * h;
     }
     const int h = h0 + r;
     if (!kSuffix && p.nsplit == 1) {
@@ -492,7 +538,7 @@ static int make_cache8_map(CUtensorMap* map, const void* cache, int num_blocks, 
   return make_tensor_map(map, cache, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <bool kSuffix>
+template <int NB, bool kSuffix>
 static int raise_smem8() {
   static std::mutex mu;
   static bool done[64];
@@ -500,14 +546,14 @@ static int raise_smem8() {
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(mu);
   if (dev < 64 && done[dev]) return NVATTN_OK;
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel<kSuffix>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel<NB, kSuffix>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, dec8_smem(NB));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_decode_fp8)");
   if (dev < 64) done[dev] = true;
   return NVATTN_OK;
 }
 
-template <bool kSuffix>
+template <int NB, bool kSuffix>
 static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
                              bool after_prefix, cudaStream_t stream) {
@@ -516,19 +562,19 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
   if (rc) return rc;
   rc = make_cache8_map(&vmap, v_cache, p.num_blocks, p.block_size, p.num_kv_heads);
   if (rc) return rc;
-  rc = raise_smem8<kSuffix>();
+  rc = raise_smem8<NB, kSuffix>();
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.nsplit, p.num_kv_heads, batch);
-  cfg.blockDim = dim3(kDecThreads);
-  cfg.dynamicSmemBytes = kSmem8;
+  cfg.blockDim = dim3((dec8_warps(NB) + 1) * 32);
+  cfg.dynamicSmemBytes = dec8_smem(NB);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = after_prefix ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_fp8_kernel<kSuffix>, kmap, vmap,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_fp8_kernel<NB, kSuffix>, kmap, vmap,
                                            k_scale, v_scale, p);
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode_fp8 launch");
 }
@@ -536,8 +582,10 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
 int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
                              bool after_prefix, cudaStream_t stream) {
-  return launch_decode_fp8<true>(p, k_cache, v_cache, k_scale, v_scale, batch, after_prefix,
-                                 stream);
+  return p.group <= 8 ? launch_decode_fp8<1, true>(p, k_cache, v_cache, k_scale, v_scale, batch,
+                                                   after_prefix, stream)
+                      : launch_decode_fp8<2, true>(p, k_cache, v_cache, k_scale, v_scale, batch,
+                                                   after_prefix, stream);
 }
 
 int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale) {
@@ -597,7 +645,9 @@ extern "C" int nvattn_paged_decode_fp8(
     return fail(NVATTN_ERR_INVALID, "paged_decode_fp8: workspace must be 256-byte aligned");
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  rc = launch_decode_fp8<false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s);
+  rc = p.group <= 8
+           ? launch_decode_fp8<1, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s)
+           : launch_decode_fp8<2, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s);
   if (rc || p.nsplit == 1) return rc;
   return launch_merge_partials(p, nullptr, nullptr, 0, batch, s);
 }
