@@ -251,9 +251,9 @@ NVATTN_API int nvattn_paged_decode_noalloc(const void* q, int64_t q_stride_tok, 
  * become zeros and set NVATTN_STATUS_BAD_BLOCK. cu_seqlens_k must not decrease.
  *
  * nvattn_paged_decode_fp8 is nvattn_paged_decode over these caches, with the
- * same sizes, limits and workspace (nvattn_decode_workspace_bytes); scores and
- * sums are fp32 and the output is rounded to bf16 once. Scales must be 16-byte
- * aligned.
+ * same sizes and limits and a workspace of nvattn_decode_fp8_workspace_bytes (0
+ * for short tables: NULL will do); scores and sums are fp32 and the output is
+ * rounded to bf16 once. Scales must be 16-byte aligned.
  */
 NVATTN_API int nvattn_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
                                         int64_t value_stride, void* k_cache, void* v_cache,
@@ -270,6 +270,11 @@ NVATTN_API int nvattn_load_kvcache_fp8(const void* k_cache, const void* v_cache,
                                        int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
                                        int64_t total_k, int32_t zero_rest, void* k_out, void* v_out,
                                        int32_t* status, void* stream);
+
+NVATTN_API size_t nvattn_decode_fp8_workspace_bytes(int32_t batch, int32_t num_heads,
+                                                    int32_t num_kv_heads,
+                                                    int32_t max_blocks_per_seq,
+                                                    int32_t block_size);
 
 NVATTN_API int nvattn_paged_decode_fp8(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
@@ -469,7 +474,7 @@ NVATTN_API int nvattn_sample_merge(const uint64_t* keys, int64_t num_shards, int
  * nodes from 0; out_tokens[b][0..a-1] = the accepted tokens, out_tokens[b][a] =
  * the drawn one; -1 behind them (everywhere, with out_num 0, in a padding row).
  * draft_tokens, u_accept (batch, nodes - 1), out_tokens and out_path (batch,
- * nodes) are contiguous. nodes <= 64, vocab <= 393216.
+ * nodes) are contiguous. nodes <= 64, vocab <= 2^20.
  */
 NVATTN_API int nvattn_verify_draft(
     const void* logits, int64_t l_stride_seq, int64_t l_stride_row, const void* draft_logits,

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(128)
       __float2bfloat16_rn(v);
 }
 
-static int device_sm_count() {
+int device_sm_count() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
   int n = 0;
@@ -392,7 +392,7 @@ void set_decode_workspace(DecodeParams* p, void* workspace, int batch) {
   p->ws_o = nullptr;
   p->ws_ml = nullptr;
   if (workspace == nullptr) return;
-  const size_t n = static_cast<size_t>(batch) * p->num_heads * p->nsplit;
+  const size_t n = static_cast<size_t>(batch) * p->num_heads * (p->nsplit / p->cluster);
   const size_t o_bytes = (n * kHeadDim * sizeof(float) + 255) & ~static_cast<size_t>(255);
   p->ws_o = static_cast<float*>(workspace);
   p->ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + o_bytes);
@@ -560,6 +560,7 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
   p.max_blocks = max_blocks_per_seq;
   p.nsplit = nsplit;
   p.split_tiles = split_tiles;
+  p.cluster = 1;
   p.key_begin = 0;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;

@@ -23,6 +23,7 @@ struct DecodeParams {
   int32_t num_blocks, block_size, num_heads, num_kv_heads, group;
   int32_t max_blocks;  // block-table width: keys past max_blocks*block_size are ignored
   int32_t nsplit, split_tiles;
+  int32_t cluster;   // fp8: splits that one cluster merges before it writes (divides nsplit)
   int32_t key_begin;  // suffix kernels: first key of the split range (a whole number of blocks)
   float scale_log2;
   float* ws_o;    // [batch][num_heads][nsplit][128]
@@ -56,9 +57,15 @@ __device__ __forceinline__ void join_prefix_grid() {
 // Split size for a batch over tables of max_blocks (see decode.cu).
 void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size, int* nsplit,
                   int* split_tiles);
+// Splits of the fp8 kernel for rows of up to max_keys, and the cluster that
+// merges them (decode_fp8.cu).
+void choose_split_fp8(int batch, int num_kv_heads, int64_t max_keys, int* nsplit, int* split_tiles,
+                      int* cluster);
+int device_sm_count();
 // Bytes of `nsplit` partials a (sequence, query head): fp32 O, then (max, sum).
 size_t decode_ws_bytes(int batch, int num_heads, int nsplit);
-// Points p.ws_o and p.ws_ml into a workspace of decode_ws_bytes (or to null).
+// Points p.ws_o and p.ws_ml into a workspace of decode_ws_bytes (or to null);
+// p.nsplit and p.cluster are set.
 void set_decode_workspace(DecodeParams* p, void* workspace, int batch);
 // Argument checks shared by the decode entry points; `who` names the caller.
 int check_decode_args(const char* who, const void* q, int64_t q_stride_tok, int64_t q_stride_head,

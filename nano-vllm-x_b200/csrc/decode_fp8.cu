@@ -20,7 +20,14 @@
 // V^T W^T): with up to 8 heads a group no MMA row and no softmax lane is
 // padding, and the conversions (2 a 4-byte word, plus one byte permute for V)
 // serve all heads. A warp owns whole 64-key tiles, the warps of a CTA taking
-// turns, so maxima, barrier waits and rescales are paid once for 64 keys.
+// turns, so maxima, barrier waits and rescales are paid once for 64 keys. Each
+// warp is its own producer: it has room for one tile of K and one of V, and
+// sends for the next tile's K as soon as the scores are out and for its V as
+// soon as the second product is, so that either half is in flight while the
+// warp works on the other. Up to 8 consecutive splits of a row form a cluster,
+// whose CTAs merge through each other's shared memory: with no more splits than
+// that the output is written at once, otherwise one fp32 partial a cluster.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -30,21 +37,27 @@
 
 namespace nvattn {
 
-constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
-constexpr int kStageBytes8 = 2 * kTile8;      // K and V
-constexpr int kScaleBytes8 = 2 * kTile;       // their exponent bytes
+namespace cg = cooperative_groups;
 
-// Consumer warps of a CTA for NB blocks of 8 query heads (registers a thread
-// grow with NB; two CTAs an SM either way). Each has one stage of the ring:
-// tile i goes to warp and stage i % warps, so a warp meets its stage's phases
-// one by one (a parity wait cannot tell phase n from n + 2, and copies may
-// land out of order).
-constexpr int dec8_warps(int NB) { return NB == 1 ? 6 : 4; }
+constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
+// Consumer warps of a CTA and CTAs of an SM for NB blocks of 8 query heads
+// (registers a thread grow with NB).
+#ifndef DEC8W
+#define DEC8W 4
+#endif
+#ifndef DEC8C
+#define DEC8C 3
+#endif
+constexpr int dec8_warps(int NB) { return NB == 1 ? DEC8W : 4; }
+constexpr int dec8_ctas(int NB) { return NB == 1 ? DEC8C : 2; }
+
+// Shared memory of one warp: its K and V tile, their exponent bytes.
+constexpr int kWarpBytes8 = 2 * kTile8;
+constexpr int kWarpScales8 = 2 * kTile;
 constexpr int dec8_smem(int NB) {
-  return dec8_warps(NB) * (kStageBytes8 + kScaleBytes8 + 2 * 8 + 8 * NB * 8) + 1024;
+  return dec8_warps(NB) * (kWarpBytes8 + kWarpScales8 + 2 * 8 + 8 * NB * 8) + 8 * NB * 8 + 1024;
 }
-static_assert(8 * kOPad * 4 <= kStageBytes8 && 16 * kOPad * 4 <= kStageBytes8,
-              "the merge buffer reuses the ring");
+static_assert(16 * kOPad * 4 <= kWarpBytes8, "the merge buffer reuses the tiles");
 
 // 1-D bulk copy into shared memory, completion on an mbarrier (16-byte
 // aligned addresses, size a multiple of 16).
@@ -132,13 +145,12 @@ __device__ __forceinline__ float load_q8(const __nv_bfloat16* row, bool live, in
 // p.key_begin on, as fp32 partials for the merge with the keys before
 // (shared_prefix.cu).
 template <int NB, bool kSuffix>
-__global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
+__global__ void __launch_bounds__(dec8_warps(NB) * 32, dec8_ctas(NB))
     paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap,
                             const uint8_t* __restrict__ k_scale,
                             const uint8_t* __restrict__ v_scale, const DecodeParams p) {
   constexpr int kWarps = dec8_warps(NB);
-  constexpr int kStages8 = kWarps;
   const int split = blockIdx.x;
   const int g = blockIdx.y;
   const int b = blockIdx.z;
@@ -150,9 +162,9 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
   const KeyRange own = kSuffix ? own_keys(p, ctx) : KeyRange{0, p.split_tiles * kTile};
   const int tok_begin = own.begin + split * own.split;
   const int tok_end = min(ctx, tok_begin + own.split);
-  if (tok_end <= tok_begin) {
+  if (tok_end <= tok_begin) {  // its cluster's other CTAs do not wait for one that ended
     if (kSuffix) join_prefix_grid();
-    if (!kSuffix && p.nsplit == 1 && split == 0) {  // no merge runs: the empty row's zeros
+    if (!kSuffix && p.nsplit == p.cluster && split == 0) {  // no merge runs: the empty row's zeros
       for (int e = threadIdx.x; e < p.group * kHeadDim; e += blockDim.x)
         p.out[static_cast<int64_t>(b) * p.o_stride_tok +
               static_cast<int64_t>(g * p.group + e / kHeadDim) * p.o_stride_head + e % kHeadDim] =
@@ -166,58 +178,48 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* scales = smem + kStages8 * kStageBytes8;
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + kStages8 * kScaleBytes8);
-  uint64_t* empty = full + kStages8;
-  float2* ml_smem = reinterpret_cast<float2*>(empty + kStages8);  // [warp][8 * NB heads]
-
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages8; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    fence_barrier_init();
-  }
-  __syncthreads();
+  uint8_t* ktile = smem + warp * kWarpBytes8;
+  uint8_t* vtile = ktile + kTile8;
+  uint8_t* ss = smem + kWarps * kWarpBytes8 + warp * kWarpScales8;  // K's bytes, then V's
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWarps * (kWarpBytes8 + kWarpScales8));
+  uint64_t* k_full = bars + 2 * warp;  // K and both rows of exponent bytes
+  uint64_t* v_full = k_full + 1;
+  float2* ml_smem = reinterpret_cast<float2*>(bars + 2 * kWarps);  // [warp][8 * NB heads]
+  float2* ml_cta = ml_smem + kWarps * 8 * NB;                      // [8 * NB heads]
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      prefetch_tensor_map(&kmap);
-      prefetch_tensor_map(&vmap);
-      const int32_t* bt = p.block_table + static_cast<int64_t>(b) * p.bt_stride;
-      int issued = 0;
-      for (; issued < ntiles; ++issued) {
-        const int stage = issued % kStages8;
-        if (!mbar_wait(&empty[stage], ((issued / kStages8) & 1) ^ 1)) {
-          set_status(p.status, NVATTN_STATUS_TIMEOUT);
-          break;
-        }
-        const int tok0 = tok_begin + issued * kTile;
-        int blk = bt[tok0 / p.block_size];
-        if (blk < 0 || blk >= p.num_blocks) {
-          set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
-          blk = 0;  // read a valid block; the result is flagged as invalid
-        }
-        const int tin = tok0 % p.block_size;
-        const int64_t sc =
-            (static_cast<int64_t>(blk) * p.num_kv_heads + g) * p.block_size + tin;
-        uint8_t* st = smem + stage * kStageBytes8;
-        uint8_t* ss = scales + stage * kScaleBytes8;
-        mbar_arrive_expect_tx(&full[stage], kStageBytes8 + kScaleBytes8);
-        tma_load_4d(st, &kmap, &full[stage], 0, g, tin, blk);
-        bulk_load(ss, k_scale + sc, kTile, &full[stage]);
-        tma_load_4d(st + kTile8, &vmap, &full[stage], 0, g, tin, blk);
-        bulk_load(ss + kTile, v_scale + sc, kTile, &full[stage]);
-      }
-      // no copy of ours is in flight when this warp ends
-      for (int it = std::max(0, issued - kStages8); it < issued; ++it)
-        mbar_wait(&full[it % kStages8], (it / kStages8) & 1);
-    }
-    return;  // the producer warp takes no part in the merge below
+  // Lane 0 sends for the warp's tiles; `blk` is the page of the tile to send
+  // for next, read from the table one tile ahead.
+  const int32_t* bt = p.block_table + static_cast<int64_t>(b) * p.bt_stride;
+  auto page = [&](int it) {
+    if (it >= ntiles) return 0;
+    const int blk = bt[(tok_begin + it * kTile) / p.block_size];
+    if (blk >= 0 && blk < p.num_blocks) return blk;
+    set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
+    return 0;  // read a valid block; the result is flagged as invalid
+  };
+  auto send_k = [&](int it, int blk) {
+    const int tin = (tok_begin + it * kTile) % p.block_size;
+    const int64_t sc = (static_cast<int64_t>(blk) * p.num_kv_heads + g) * p.block_size + tin;
+    mbar_arrive_expect_tx(k_full, kTile8 + kWarpScales8);
+    tma_load_4d(ktile, &kmap, k_full, 0, g, tin, blk);
+    bulk_load(ss, k_scale + sc, kTile, k_full);
+    bulk_load(ss + kTile, v_scale + sc, kTile, k_full);
+  };
+  auto send_v = [&](int it, int blk) {
+    mbar_arrive_expect_tx(v_full, kTile8);
+    tma_load_4d(vtile, &vmap, v_full, 0, g, (tok_begin + it * kTile) % p.block_size, blk);
+  };
+  if (lane == 0 && warp < ntiles) {
+    mbar_init(k_full, 1);
+    mbar_init(v_full, 1);
+    fence_barrier_init();
+    const int blk = page(warp);
+    send_k(warp, blk);
+    send_v(warp, blk);
   }
+  __syncwarp();
 
   // -------------------------------------------------------------- consumers
   const int quad = lane & 3;  // this lane's head columns 2*quad, 2*quad + 1 of each block
@@ -254,18 +256,18 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
 #pragma unroll
   for (int i = 0; i < 4; ++i) off[i] = swz128(lane & 15, 2 * i + (lane >> 4));
 
+  const uint32_t kbase = smem_u32(ktile), vbase = smem_u32(vtile);
   bool timed_out = false;
-  for (int it = warp; it < ntiles; it += kWarps) {
-    const int stage = it % kStages8;
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (it / kStages8) & 1))) {
+  uint32_t phase = 0;
+  for (int it = warp; it < ntiles; it += kWarps, phase ^= 1) {
+    const int next = it + kWarps;
+    int next_blk = 0;
+    if (lane == 0) next_blk = page(next);
+    if (!__all_sync(0xffffffffu, mbar_wait(k_full, phase))) {
       timed_out = true;
       break;
     }
     const int nvalid = min(kTile, tok_end - (tok_begin + it * kTile));
-    uint8_t* st = smem + stage * kStageBytes8;
-    const uint8_t* ss = scales + stage * kScaleBytes8;
-    const uint32_t kbase = smem_u32(st);
-    const uint32_t vbase = kbase + kTile8;
     // ---- S^T = K Q^T: 4 steps of 16 keys, 8 of 16 dims
     float s[4][NB][4];  // [mt][nb][2e + j]: key 16mt + 8e + sub, head column 2*quad + j
 #pragma unroll
@@ -306,13 +308,9 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
         }
       }
     }
-    if (nvalid < kTile) {
-      // Keys past the end hold stale bytes (maybe NaN): their scores are
-      // masked, and their V rows zeroed so that 0 * NaN never reaches the sum.
-      // Only a range's last tile has them, so no later copy lands in this
-      // stage.
-      for (int e = lane; e < (kTile - nvalid) * 8; e += 32)
-        *reinterpret_cast<int4*>(st + kTile8 + nvalid * 128 + e * 16) = make_int4(0, 0, 0, 0);
+    __syncwarp();  // K and the exponents are read: the next tile's may land
+    if (lane == 0 && next < ntiles) send_k(next, next_blk);
+    if (nvalid < kTile) {  // keys past the end: stale bytes
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
@@ -324,7 +322,6 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
           }
         }
       }
-      __syncwarp();
     }
     float mn[NB][2];
     bool grew = false;
@@ -363,6 +360,17 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
       }
     }
     // ---- O^T += V^T W^T: 4 steps of 16 keys
+    if (!__all_sync(0xffffffffu, mbar_wait(v_full, phase))) {
+      timed_out = true;
+      break;
+    }
+    if (nvalid < kTile) {
+      // Zero the V rows past the end (maybe NaN), so that 0 * NaN never reaches
+      // the sum. Only a range's last tile has them: no later copy lands here.
+      for (int e = lane; e < (kTile - nvalid) * 8; e += 32)
+        *reinterpret_cast<int4*>(vtile + nvalid * 128 + e * 16) = make_int4(0, 0, 0, 0);
+      __syncwarp();
+    }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       uint32_t wb[NB][2];
@@ -395,13 +403,17 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[stage]);
+    if (lane == 0 && next < ntiles) send_v(next, next_blk);
   }
-  if (timed_out && lane == 0) set_status(p.status, NVATTN_STATUS_TIMEOUT);
+  if (timed_out) {  // the copies in flight, again with a limit
+    mbar_wait(k_full, phase);
+    mbar_wait(k_full, phase ^ 1);
+    mbar_wait(v_full, phase);
+    if (lane == 0) set_status(p.status, NVATTN_STATUS_TIMEOUT);
+  }
 
   // ---------------------------------------------------------------- merge
-  // All consumer warps are past their last ring read: reuse the ring.
-  asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32));
+  __syncthreads();  // all warps are past their tiles: reuse them
   float* obuf = reinterpret_cast<float*>(smem);  // [warp][8 * NB heads][kOPad]
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -419,8 +431,23 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
             make_float2(o[c][nb][j], o[c][nb][2 + j]);
     }
   }
-  asm volatile("bar.sync 1, %0;" ::"r"(kWarps * 32));
+  __syncthreads();
 
+  const int first = split - split % p.cluster;
+  const int live = min(p.cluster, (ctx - own.begin + own.split - 1) / own.split - first);
+  const int64_t slot0 = (static_cast<int64_t>(b) * p.num_heads + h0) * (p.nsplit / p.cluster) +
+                        split / p.cluster;
+  auto put = [&](int r, int d, float mmax, float L, float acc) {
+    if (!kSuffix && p.nsplit == p.cluster) {
+      p.out[static_cast<int64_t>(b) * p.o_stride_tok +
+            static_cast<int64_t>(h0 + r) * p.o_stride_head + d] = __float2bfloat16_rn(acc / L);
+    } else {
+      const int64_t slot = slot0 + static_cast<int64_t>(r) * (p.nsplit / p.cluster);
+      p.ws_o[slot * kHeadDim + d] = acc;
+      if (d == 0) p.ws_ml[slot] = make_float2(mmax, L);
+    }
+  };
+  // over the CTA's warps, in place: element (r, d) is one thread's
   for (int e = threadIdx.x; e < p.group * kHeadDim; e += kWarps * 32) {
     const int r = e / kHeadDim, d = e % kHeadDim;
     float mmax = neg_inf();
@@ -435,72 +462,104 @@ __global__ void __launch_bounds__((dec8_warps(NB) + 1) * 32, 2)
       L += ml.y * h * h;
       acc += obuf[(w * 8 * NB + r) * kOPad + d] * h * h;
     }
-    const int h = h0 + r;
-    if (!kSuffix && p.nsplit == 1) {
-      p.out[static_cast<int64_t>(b) * p.o_stride_tok + static_cast<int64_t>(h) * p.o_stride_head +
-            d] = __float2bfloat16_rn(acc / L);
+    if (live == 1) {
+      put(r, d, mmax, L, acc);
     } else {
-      const int64_t slot = (static_cast<int64_t>(b) * p.num_heads + h) * p.nsplit + split;
-      p.ws_o[slot * kHeadDim + d] = acc;
-      if (d == 0) p.ws_ml[slot] = make_float2(mmax, L);
+      obuf[r * kOPad + d] = acc;
+      if (d == 0) ml_cta[r] = make_float2(mmax, L);
     }
   }
+  if (live == 1) {
+    if (kSuffix) join_prefix_grid();
+    return;
+  }
+  // over the cluster's splits that have keys: the first ones
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int e = (split - first) * kWarps * 32 + threadIdx.x; e < p.group * kHeadDim;
+       e += live * kWarps * 32) {
+    const int r = e / kHeadDim, d = e % kHeadDim;
+    float mmax = neg_inf();
+    for (int c = 0; c < live; ++c) mmax = fmaxf(mmax, cluster.map_shared_rank(ml_cta, c)[r].x);
+    float L = 0.f, acc = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < live; ++c) {
+      const float2 ml = cluster.map_shared_rank(ml_cta, c)[r];
+      const float h = (ml.x == neg_inf()) ? 0.f : fast_exp2(0.5f * (ml.x - mmax));
+      L += ml.y * h * h;
+      acc += cluster.map_shared_rank(obuf, c)[r * kOPad + d] * h * h;
+    }
+    put(r, d, mmax, L, acc);
+  }
+  cluster.sync();  // no CTA ends while the others read from it
   if (kSuffix) join_prefix_grid();
 }
 
-// Merges the partials of one (sequence, query head) per warp: lane i owns dims
-// 4i..4i+3. Launched as a programmatic dependent of the kernel that writes the
-// last partials.
-constexpr int kMergeWarps = 4;
+// Merges the partials of one (sequence, query head), W warps a row: lane i owns
+// dims 4i..4i+3, a warp every W-th partial. Launched as a programmatic
+// dependent of the kernel that writes the last partials. Latency-bound: a warp
+// has four partials in flight, so many partials want several warps a row.
+constexpr int kMergeThreads = 256;
 
-__global__ void __launch_bounds__(kMergeWarps * 32)
+template <int W>
+__global__ void __launch_bounds__(kMergeThreads)
     merge_partials_kernel(const DecodeParams p, const float* __restrict__ first_o,
                           const float2* __restrict__ first_ml, int nfirst, int rows) {
+  constexpr int kRows = kMergeThreads / 32 / W;
+  __shared__ float4 part[W > 1 ? kMergeThreads : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wr = warp % W;
+  const int row = min(static_cast<int>(blockIdx.x) * kRows + warp / W, rows - 1);
   const int b = row / p.num_heads, h = row - b * p.num_heads;
   const int ctx = min(p.seqlens[b], p.max_blocks * p.block_size);
   const KeyRange own = own_keys(p, ctx);
   const int nf = own.begin > 0 ? nfirst : 0;
-  const int n = nf + min(p.nsplit, (max(ctx - own.begin, 0) + own.split - 1) / own.split);
+  const int nparts = p.nsplit / p.cluster, part_keys = own.split * p.cluster;
+  const int n = nf + min(nparts, (max(ctx - own.begin, 0) + part_keys - 1) / part_keys);
   // partials 0..nf-1 are the first range's, nf..n-1 the own ones
   const int64_t fbase = static_cast<int64_t>(row) * nfirst;
-  const int64_t obase = static_cast<int64_t>(row) * p.nsplit;
-  auto ml_at = [&](int s) { return s < nf ? first_ml[fbase + s] : p.ws_ml[obase + s - nf]; };
+  const int64_t obase = static_cast<int64_t>(row) * nparts - nf;
+  auto ml_at = [&](int s) { return s < nf ? first_ml[fbase + s] : p.ws_ml[obase + s]; };
   float mmax = neg_inf();
   for (int s = lane; s < n; s += 32) mmax = fmaxf(mmax, ml_at(s).x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1)
     mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, off));
+  // half steps, as in the kernels: l times the factor stays in range
+  auto half = [&](float m) { return m == neg_inf() ? 0.f : fast_exp2(0.5f * (m - mmax)); };
   float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    float wt = 0.f;
-    if (s0 + lane < n) {
-      const float2 ml = ml_at(s0 + lane);
-      // half steps, as in the kernels: l times the factor stays in range
-      const float hw = (ml.x == neg_inf()) ? 0.f : fast_exp2(0.5f * (ml.x - mmax));
-      L += ml.y * hw * hw;
-      wt = hw * hw;
-    }
-    const int cnt = min(32, n - s0);
-#pragma unroll 4
-    for (int i = 0; i < cnt; ++i) {
-      const int s = s0 + i;
-      const float* src = s < nf ? first_o + (fbase + s) * kHeadDim
-                                : p.ws_o + (obase + s - nf) * kHeadDim;
-      const float4 o = reinterpret_cast<const float4*>(src)[lane];
-      const float w = __shfl_sync(0xffffffffu, wt, i);
-      acc.x += o.x * w;
-      acc.y += o.y * w;
-      acc.z += o.z * w;
-      acc.w += o.w * w;
-    }
+  for (int s = lane; s < n; s += 32) {
+    const float2 ml = ml_at(s);
+    const float hw = half(ml.x);
+    L += ml.y * hw * hw;
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = wr; s < n; s += W) {
+    const float* src = s < nf ? first_o + (fbase + s) * kHeadDim : p.ws_o + (obase + s) * kHeadDim;
+    const float4 o = reinterpret_cast<const float4*>(src)[lane];
+    const float hw = half(ml_at(s).x), w = hw * hw;
+    acc.x += o.x * w;
+    acc.y += o.y * w;
+    acc.z += o.z * w;
+    acc.w += o.w * w;
+  }
+  if (W > 1) {
+    part[threadIdx.x] = acc;
+    __syncthreads();
+    if (wr != 0) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float4 o = part[threadIdx.x + 32 * i];
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+    }
+  }
   const float inv = n > 0 ? 1.f / L : 0.f;  // a row without keys: zeros
   __nv_bfloat16* out = p.out + static_cast<int64_t>(b) * p.o_stride_tok +
                        static_cast<int64_t>(h) * p.o_stride_head + lane * 4;
@@ -512,18 +571,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 int launch_merge_partials(const DecodeParams& p, const float* first_o, const float2* first_ml,
                           int nfirst, int batch, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(batch) * p.num_heads;
-  if (rows > 0x7fffffffLL - kMergeWarps) return fail(NVATTN_ERR_INVALID, "decode: too many rows");
+  if (rows > 0x7fffffffLL - kMergeThreads)
+    return fail(NVATTN_ERR_INVALID, "decode: too many rows");
+  const bool wide = nfirst + p.nsplit / p.cluster > 16;
+  const int per_cta = wide ? 1 : kMergeThreads / 32;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + kMergeWarps - 1) / kMergeWarps));
-  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta));
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, merge_partials_kernel, p, first_o, first_ml,
-                                           nfirst, static_cast<int>(rows));
+  const cudaError_t e =
+      wide ? cudaLaunchKernelEx(&cfg, merge_partials_kernel<kMergeThreads / 32>, p, first_o,
+                                first_ml, nfirst, static_cast<int>(rows))
+           : cudaLaunchKernelEx(&cfg, merge_partials_kernel<1>, p, first_o, first_ml, nfirst,
+                                static_cast<int>(rows));
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "merge_partials launch");
 }
 
@@ -566,14 +631,17 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.nsplit, p.num_kv_heads, batch);
-  cfg.blockDim = dim3((dec8_warps(NB) + 1) * 32);
+  cfg.blockDim = dim3(dec8_warps(NB) * 32);
   cfg.dynamicSmemBytes = dec8_smem(NB);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = after_prefix ? 1 : 0;
+  cfg.numAttrs = after_prefix ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_fp8_kernel<NB, kSuffix>, kmap, vmap,
                                            k_scale, v_scale, p);
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode_fp8 launch");
@@ -588,6 +656,30 @@ int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const v
                                                    after_prefix, stream);
 }
 
+// Splits of a row, in 64-key tiles: the largest of 32/16/8/4 that gives 8 CTAs
+// an SM when every row is at the table's width; a batch too small for that
+// keeps 8 where they still cover the SMs once (two tiles a warp), and 4 (one)
+// otherwise. A batch whose splits all run at once merges them in clusters of up
+// to 8. Depends on host sizes only, so a captured graph keeps its grid.
+void choose_split_fp8(int batch, int num_kv_heads, int64_t max_keys, int* nsplit,
+                      int* split_tiles, int* cluster) {
+  const int sms = device_sm_count();
+  const int64_t tiles = std::max<int64_t>(1, (max_keys + kTile - 1) / kTile);
+  const int64_t pairs = static_cast<int64_t>(batch) * num_kv_heads;
+  int st = 32;
+  while (st > 4 && pairs * ((tiles + st - 1) / st) < (st > 8 ? 8 : 1) * static_cast<int64_t>(sms))
+    st >>= 1;
+  const int64_t ns = (tiles + st - 1) / st;
+  // Clusters save the merge's launch and its reads (1 x 777 keys: 6.4 -> 5.6 us),
+  // but their CTAs wait for one another: with more CTAs than the SMs hold at
+  // once that keeps others from starting (32 long contexts: 179 -> 194 us).
+  int c = 1;
+  while (pairs * ns <= 2 * static_cast<int64_t>(sms) && c < 8 && c < ns) c *= 2;
+  *split_tiles = st;
+  *cluster = c;
+  *nsplit = static_cast<int>((ns + c - 1) / c * c);
+}
+
 int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale) {
   if (!k_scale || !v_scale) return fail(NVATTN_ERR_INVALID, std::string(who) + ": NULL scales");
   if (!aligned16(k_scale) || !aligned16(v_scale))
@@ -598,6 +690,20 @@ int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale) 
 }  // namespace nvattn
 
 using namespace nvattn;
+
+extern "C" size_t nvattn_decode_fp8_workspace_bytes(int32_t batch, int32_t num_heads,
+                                                    int32_t num_kv_heads,
+                                                    int32_t max_blocks_per_seq,
+                                                    int32_t block_size) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_blocks_per_seq <= 0 ||
+      block_size <= 0)
+    return 0;
+  int nsplit, split_tiles, cluster;
+  choose_split_fp8(batch, num_kv_heads,
+                   static_cast<int64_t>(max_blocks_per_seq) * block_size, &nsplit, &split_tiles,
+                   &cluster);
+  return decode_ws_bytes(batch, num_heads, nsplit / cluster);
+}
 
 extern "C" int nvattn_paged_decode_fp8(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
@@ -636,11 +742,13 @@ extern "C" int nvattn_paged_decode_fp8(
   p.max_blocks = max_blocks_per_seq;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;
-  choose_split(batch, num_kv_heads, max_blocks_per_seq, block_size, &p.nsplit, &p.split_tiles);
-  const size_t need = decode_ws_bytes(batch, num_heads, p.nsplit);
+  choose_split_fp8(batch, num_kv_heads,
+                   static_cast<int64_t>(max_blocks_per_seq) * block_size, &p.nsplit,
+                   &p.split_tiles, &p.cluster);
+  const size_t need = decode_ws_bytes(batch, num_heads, p.nsplit / p.cluster);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(NVATTN_ERR_WORKSPACE, "paged_decode_fp8: workspace smaller than "
-                                      "nvattn_decode_workspace_bytes()");
+                                      "nvattn_decode_fp8_workspace_bytes()");
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(NVATTN_ERR_INVALID, "paged_decode_fp8: workspace must be 256-byte aligned");
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
@@ -648,6 +756,6 @@ extern "C" int nvattn_paged_decode_fp8(
   rc = p.group <= 8
            ? launch_decode_fp8<1, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s)
            : launch_decode_fp8<2, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s);
-  if (rc || p.nsplit == 1) return rc;
+  if (rc || p.nsplit == p.cluster) return rc;
   return launch_merge_partials(p, nullptr, nullptr, 0, batch, s);
 }

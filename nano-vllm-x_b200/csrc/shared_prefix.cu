@@ -25,7 +25,7 @@ static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255);
 // Byte offsets of the workspace's regions and the splits they hold.
 struct SharedLayout {
   int np, ptiles;  // splits of the prefix (0: no prefix)
-  int ns, stiles;  // splits of the own keys
+  int ns, stiles, cluster;  // splits of the own keys; those that a cluster merges
   size_t prefix_o, prefix_ml, own, k, v, bytes;
 };
 
@@ -34,8 +34,13 @@ static SharedLayout shared_layout(int batch, int num_heads, int num_kv_heads, in
   SharedLayout w{};
   if (shared_len > 0)
     shared_split(batch, num_heads, num_kv_heads, shared_len, &w.np, &w.ptiles);
-  choose_split(batch, num_kv_heads, std::max(1, max_blocks - shared_len / block_size), block_size,
-               &w.ns, &w.stiles);
+  const int own_blocks = std::max(1, max_blocks - shared_len / block_size);
+  w.cluster = 1;
+  if (fp8)
+    choose_split_fp8(batch, num_kv_heads, static_cast<int64_t>(own_blocks) * block_size, &w.ns,
+                     &w.stiles, &w.cluster);
+  else
+    choose_split(batch, num_kv_heads, own_blocks, block_size, &w.ns, &w.stiles);
   const size_t rows = static_cast<size_t>(batch) * num_heads;
   size_t at = 0;
   w.prefix_o = at;
@@ -43,7 +48,8 @@ static SharedLayout shared_layout(int batch, int num_heads, int num_kv_heads, in
   w.prefix_ml = at;
   at += round256(rows * w.np * sizeof(float2));
   w.own = at;
-  at += round256(rows * w.ns * kHeadDim * sizeof(float)) + round256(rows * w.ns * sizeof(float2));
+  const size_t parts = rows * (w.ns / w.cluster);
+  at += round256(parts * kHeadDim * sizeof(float)) + round256(parts * sizeof(float2));
   if (fp8) {
     const size_t kv = static_cast<size_t>(shared_len) * num_kv_heads * kHeadDim * 2;
     w.k = at;
@@ -129,6 +135,7 @@ extern "C" int nvattn_shared_prefix_decode(
   p.max_blocks = max_blocks_per_seq;
   p.nsplit = w.ns;
   p.split_tiles = w.stiles;
+  p.cluster = w.cluster;
   p.key_begin = shared_len;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;

@@ -61,6 +61,7 @@ SIGNATURES: dict[str, tuple] = {
     "nvattn_load_kvcache_fp8": (c_int, [_P, _P, _P, _P, _I32P, c_int32, _I32P, c_int64, c_int32,
                                         c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, _P, _P,
                                         _I32P, _P]),
+    "nvattn_decode_fp8_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "nvattn_paged_decode_fp8": (c_int, [_P, c_int64, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64,
                                         _I32P, _I32P, c_int64, c_int32, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int32, c_float, _P, c_size_t,
@@ -142,7 +143,7 @@ def load(path: os.PathLike | str | None = None) -> ctypes.CDLL:
 
 def call(name: str, *args) -> int:
     """Call entry point `name`; raise NvattnError on a non-zero code."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != OK:
         msg = lib.nvattn_last_error().decode(errors="replace")

@@ -57,6 +57,7 @@ __all__ = [
     "sample_merge",
     "verify_draft",
     "decode_workspace_bytes",
+    "decode_fp8_workspace_bytes",
     "tree_workspace_bytes",
     "status_tensor",
     "read_status",
@@ -124,7 +125,14 @@ def _status_ptr(device: torch.device) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# torch's accessor of the current stream's handle, without the Stream object
+# that torch.cuda.current_stream builds (2.5 us of a call's host time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -177,7 +185,7 @@ def _check_decode(q: torch.Tensor, out: torch.Tensor | None, cache_seqlens: torc
     if cache_seqlens.numel() != batch:
         raise ValueError("cache_seqlens must have one entry per row of q")
     if out is None:
-        out = torch.empty((batch, num_heads, head_dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.stride(2) != 1:
         raise ValueError("out must have q's shape and a contiguous last dimension")
     return batch, num_heads, head_dim, out
@@ -467,6 +475,12 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     return k_out, v_out
 
 
+def decode_fp8_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, max_blocks: int,
+                               block_size: int) -> int:
+    return int(_lib.load().nvattn_decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads,
+                                                             max_blocks, block_size))
+
+
 def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                      k_scale: torch.Tensor, v_scale: torch.Tensor, cache_seqlens: torch.Tensor,
                      block_table: torch.Tensor, softmax_scale: float | None = None,
@@ -474,7 +488,7 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_decode`` over an fp8 cache (``store_kvcache_fp8``); q, out: (B, H, d) bf16.
 
-    ``workspace``: uint8, ``decode_workspace_bytes`` of the same sizes.
+    ``workspace``: uint8, ``decode_fp8_workspace_bytes`` of the same sizes.
     """
     dev = _require_cuda(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, out,
                         workspace)
@@ -483,8 +497,8 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                                                     num_kv_heads, k_cache.shape[3])
     max_blocks = block_table.shape[1]
     with _device(dev):
-        ws_ptr, ws_bytes = _workspace(decode_workspace_bytes(batch, num_heads, num_kv_heads,
-                                                             max_blocks, block_size),
+        ws_ptr, ws_bytes = _workspace(decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads,
+                                                                 max_blocks, block_size),
                                       workspace, dev)
         _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

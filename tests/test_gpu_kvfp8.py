@@ -228,7 +228,7 @@ def test_decode_empty_rows_give_zeros():
     check(out, ref, mag)
     # one split covers the table: the kernel itself writes the zeros
     lens = [0, 200] * 300
-    assert ops.decode_workspace_bytes(600, 4, 2, 1, 256) == 0
+    assert ops.decode_fp8_workspace_bytes(600, 4, 2, 1, 256) == 0
     out, ref, mag = _decode(lens, 4, 2, seed=3)
     assert (out[::2] == 0).all()
     check(out, ref, mag)

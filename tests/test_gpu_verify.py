@@ -184,7 +184,7 @@ def test_strided_and_unaligned_rows():
 
 def test_largest_vocabulary_and_one_column():
     for form in ("chain", "draft"):
-        _check(*_inputs(2, 3, 393216, 18, form))
+        _check(*_inputs(2, 3, 1 << 20, 18, form))
         x, tok, u, pick, kw = _inputs(2, 3, 1, 19, form, hot=1)
         _check(x, tok, u, pick, kw)
 

@@ -81,7 +81,7 @@ def test_c_refusals():
                            (dict(tok=None), _lib.ERR_INVALID, b"NULL"),
                            (dict(nodes=65), _lib.ERR_UNSUPPORTED, b"64 nodes"),
                            (dict(vocab=0), _lib.ERR_INVALID, b"vocab"),
-                           (dict(vocab=393217), _lib.ERR_UNSUPPORTED, b"393216"),
+                           (dict(vocab=2 ** 20 + 1), _lib.ERR_UNSUPPORTED, b"2^20"),
                            (dict(draft=FAKE, parents=FAKE), _lib.ERR_UNSUPPORTED, b"chain"),
                            (dict(stride=-1), _lib.ERR_INVALID, b"negative stride"),
                            (dict(logits=ctypes.c_void_p(0x10001)), _lib.ERR_INVALID, b"2-byte"),
