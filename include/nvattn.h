@@ -466,8 +466,9 @@ NVATTN_API int nvattn_sample_merge(const uint64_t* keys, int64_t num_shards, int
  * cumulative weight exceeds u_pick[b] * total, in column order; where rounding
  * leaves no weight it is from p. temperatures NULL or <= 0: greedy, a child is
  * accepted iff its token is the argmax (first index on ties), which is also the
- * draw. NaN and -inf logits have no probability, an infinite one all of it; a
- * row with nothing else accepts nothing and gives column 0. A drafted token
+ * draw (above 1e30 they count as 1e30). NaN and -inf logits have no probability, an infinite one all of it; a
+ * row with nothing else accepts nothing and gives column 0. A probability below
+ * 2^-950 of its row's largest counts as none. A drafted token
  * outside [0, vocab) is rejected. Decisions are those of 64-bit arithmetic.
  *
  * out_num[b] = number of accepted drafts a; out_path[b][0..a] = the walked

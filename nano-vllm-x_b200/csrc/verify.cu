@@ -17,12 +17,15 @@
 // token whose cumulative weight exceeds u * total. T <= 0: a child is accepted
 // iff it is the argmax, the draw is the argmax.
 //
-// Only the rows on the walked path are read: one cluster of CTAs per sequence
-// walks it, a CTA per slice of the columns, and every CTA takes the same
-// decisions from the same exchanged sums. Scanning a row costs one MUFU
+// Two kernels. The walk reads only the rows on the path: one cluster of CTAs per
+// sequence, a CTA per slice of the columns. A row costs one pass with one MUFU
 // exponential and about four other instructions a logit (each thread sums
-// against its own maximum, so a row is read once and nothing is staged); the
-// exchange is one cluster barrier a node.
+// against its own maximum) and one cluster barrier: every warp writes its sums
+// into the shared memory of all CTAs, and after the barrier every warp adds the
+// same numbers up and takes the same decision, with nothing to broadcast. It is
+// kept to 64 registers and short code: rows are a chain, so what hides their
+// latency is other sequences on the same SM. The draw then goes over each
+// sequence's last row, all sequences at once.
 //
 // The answers are tokens, so sums that decide between neighbours are kept in
 // 64 bits: the draw's cumulative weights always (with 151,936 weights of which
@@ -31,14 +34,14 @@
 // within 2^-14 of the border. 2^t in fp64 is table-driven (P. T. P. Tang, ACM
 // TOMS 15(2), 1989): t = k/1024 + f, |f| <= 2^-11, 2^t = 2^(k>>10) *
 // T[k & 1023] * 2^f with a cubic (error (f ln 2)^4/24 < 6e-16), 8 fp64
-// operations. The draw reads its row a second time (from L2) for those sums: a
-// lane owns a run of columns, so prefix sums over lanes, warps and CTAs find
-// the lane whose run crosses the threshold, and one warp scans that run.
+// operations, which bound the draw. In it a warp owns consecutive columns, its
+// lanes keep the sums of consecutive bins, and prefix sums over warps, bins and
+// lanes find the column.
 #include <cooperative_groups.h>
 
 #include <mutex>
 
-#include "common.cuh"
+#include "decode.cuh"
 
 namespace nvattn {
 
@@ -50,6 +53,10 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxNodes = 64;
 constexpr int kMaxVocab = 1 << 20;  // keeps the fp32 sums well inside decide()'s margin
 constexpr int kExpTable = 1024;
+constexpr uint32_t kNoLogit = 0xff80u;  // bf16 bits of -inf
+// Temperatures count up to this (every law is flat long before): a logit of
+// -inf is then 2^-980 below any other, and never drawn.
+constexpr float kMaxTemperature = 1e30f;
 
 struct VerifyParams {
   const __nv_bfloat16* logits;
@@ -69,28 +76,34 @@ struct VerifyParams {
   int32_t* out_num;
 };
 
-// What a CTA tells the others of its slice.
-struct VerifySums {
-  unsigned long long key;  // largest logit and its first column (vkey order)
-  float qmax;
-  double psum, qsum;       // sums of exponentials, or of weights
+// What a warp tells the cluster: (max, sum) of its part of the target's and the
+// draft's row; or a pick key; or two fp64 sums.
+union VerifySlot {
+  float4 f;
+  double2 d;
+  unsigned long long key[2];
 };
 
 struct VerifyShared {
-  VerifySums sums[2];
-  double warp_a[kVerifyWarps], warp_b[kVerifyWarps];
-  unsigned long long warp_key[kVerifyWarps];
-  float warp_q[kVerifyWarps];
-  // the cluster's totals
-  float pmax, qmax;
-  int argmax, owner;
-  double psum, qsum, base;
-  int32_t parents[kMaxNodes];
-  int next, count, nrejected, open;
-  int32_t path[kMaxNodes + 1];
-  int64_t rejected[kMaxNodes];
-  double table[kExpTable];
+  VerifySlot slots[2][kMaxCluster * kVerifyWarps];  // of all warps, in column order
 };
+
+// What the walk leaves in out_tokens[b][count] for the draw, which overwrites it
+// with the token: the largest logits of the last row (bf16 bits) and the ratio
+// of its sums of exponentials, target over draft.
+struct DrawState {
+  uint32_t top, qtop;
+  float ratio;
+};
+__device__ __forceinline__ int64_t pack_state(const DrawState& s) {
+  return static_cast<int64_t>((static_cast<uint64_t>(__float_as_uint(s.ratio)) << 32) |
+                              (s.qtop << 16) | s.top);
+}
+__device__ __forceinline__ DrawState unpack_state(int64_t v) {
+  const uint64_t u = static_cast<uint64_t>(v);
+  return {static_cast<uint32_t>(u) & 0xffffu, (static_cast<uint32_t>(u) >> 16),
+          __uint_as_float(static_cast<uint32_t>(u >> 32))};
+}
 
 __device__ __forceinline__ unsigned long long vkey(float s, uint32_t col) {
   uint32_t b = __float_as_uint(s == 0.f ? 0.f : s);
@@ -103,18 +116,50 @@ __device__ __forceinline__ float vkey_score(unsigned long long key) {
   return key == 0ull ? -INFINITY : __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
-// fp64 value of a bf16 (zero and subnormals become +-2^-127 and above, far
-// below any logit's spacing that matters).
-__device__ __forceinline__ double bf16_to_f64(uint32_t b) {
-  const uint32_t hi = ((b & 0x8000u) << 16) | (((b & 0x7fffu) << 13) + (896u << 20));
-  return __hiloint2double(static_cast<int>(hi), 0);
+// exp2 of j / 1024 for a CTA's table.
+__device__ __forceinline__ void fill_table(double* table) {
+  for (int i = threadIdx.x; i < kExpTable; i += kVerifyThreads)
+    table[i] = exp2(static_cast<double>(i) / kExpTable);
 }
 
-// 2^((l - top) * c) in fp64 for a bf16 logit that is not NaN: exactly 1 for the
-// largest (also where that is infinite), exactly 0 below 2^-1000.
-__device__ __forceinline__ double weight64(uint32_t bits, uint32_t top_bits, double c, double top_c,
-                                           const double* __restrict__ table) {
-  const double t = fma(bf16_to_f64(bits), c, -top_c);
+// One row's scale in fp64: the weight of a bf16 logit l is 2^((l - top) * c),
+// held above 2^-1000 (no draw reaches weights below kNothing). c is at most what
+// puts the next bf16 below the top at 2^-2000, so that top * c stays small
+// enough for its rounding. Rows whose largest logit is infinite are weighed as 0
+// for an infinite logit and -980 for any other, with c = 1.
+struct RowScale {
+  double c, top_c;
+  bool inf;
+
+  __device__ __forceinline__ RowScale(uint32_t top_bits, double c64) {
+    const float top = __uint_as_float(top_bits << 16);
+    inf = top_bits == 0x7f80u;
+    const uint32_t below = (top_bits & 0x7fffu) == 0u ? 0x8001u
+                           : (top_bits & 0x8000u)     ? top_bits + 1u
+                                                      : top_bits - 1u;
+    const double gap = static_cast<double>(top) - static_cast<double>(__uint_as_float(below << 16));
+    c = inf ? 1.0 : fmin(c64, 2000.0 / gap);
+    top_c = inf ? 0.0 : static_cast<double>(top) * c;
+  }
+  // NaN and -inf become the lowest bf16.
+  __device__ __forceinline__ uint32_t raise(uint32_t two) const {
+    if (inf)
+      two = ((two & 0xffffu) == 0x7f80u ? 0u : 0xc475u) |
+            ((two >> 16) == 0x7f80u ? 0u : 0xc4750000u);  // -980
+    const __nv_bfloat162 lowest(__nv_bfloat162_raw{0xff7fu, 0xff7fu});
+    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&two), lowest);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ double log2_weight(float l) const {
+    const double t = fma(static_cast<double>(l), c, -top_c);
+    // max(t, -1000) on the high word: as unsigned, further below zero is larger
+    const uint32_t hi = min(static_cast<uint32_t>(__double2hiint(t)), 0xC08F4000u);
+    return __hiloint2double(static_cast<int>(hi), __double2loint(t));
+  }
+};
+
+// 2^t for t in [-1001, 1].
+__device__ __forceinline__ double exp2_64(double t, const double* __restrict__ table) {
   const double shift = 6597069766656.0;  // 1.5 * 2^42: rounds to multiples of 2^-10
   const double s = t + shift;
   const int k = __double2loint(s);
@@ -123,16 +168,37 @@ __device__ __forceinline__ double weight64(uint32_t bits, uint32_t top_bits, dou
   e = fma(e, f, 0.69314718055994531);
   const double tj = table[k & (kExpTable - 1)];
   const double r = fma(e * f, tj, tj);
-  const double w = __hiloint2double(__double2hiint(r) + ((k >> 10) << 20), __double2loint(r));
-  // t's high word as an integer: -1000 and below
-  const bool none = static_cast<uint32_t>(__double2hiint(t)) >= 0xC08F4000u || bits == 0xff80u;
-  return bits == top_bits ? 1.0 : (none ? 0.0 : w);
+  return __hiloint2double(__double2hiint(r) + ((k & ~(kExpTable - 1)) << 10), __double2loint(r));
 }
+
+// Weights up to this count as none: above the sum of all that log2_weight held
+// up (2^20 columns of 2^-980 at most). Thresholds are raised to it.
+constexpr double kNothing = 0x1p-950;
 
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T warp_max(T v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const T w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// Inclusive prefix sum over the lanes.
+__device__ __forceinline__ double warp_scan(double v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
   return v;
 }
 
@@ -148,70 +214,84 @@ __device__ __forceinline__ uint32_t clean2(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Columns [at, at + 8) of a slice of `len` columns as 4 pairs, -inf outside the
-// slice and for NaN; one 16-byte load where the address allows.
-__device__ __forceinline__ void load8(const unsigned short* src, int at, int len, uint32_t w[4]) {
-  if (at >= 0 && at + 8 <= len && (reinterpret_cast<uintptr_t>(src + at) & 15) == 0) {
-    const int4 v = __ldg(reinterpret_cast<const int4*>(src + at));
+// Columns [0, len) of a row at `src`, as 16-byte groups at the row's own
+// alignment: group g holds columns 8g - shift .. 8g - shift + 7. Groups [lo, hi)
+// lie inside and are one load each; one before and one behind may lie partly
+// inside and are read element by element.
+struct Slice {
+  const unsigned short* src;
+  int len, shift, lo, hi, groups;
+
+  __device__ __forceinline__ Slice(const unsigned short* s, int n)
+      : src(s),
+        len(n),
+        shift(static_cast<int>((reinterpret_cast<uintptr_t>(s) & 15) >> 1)),
+        lo(shift > 0 ? 1 : 0),
+        hi((shift + n) / 8),
+        groups((shift + n + 7) / 8) {}
+
+  // Issues group g's load, if it lies inside (-inf otherwise); nothing here
+  // depends on the data, so a batch of these is in flight together.
+  __device__ __forceinline__ void load(int g, uint32_t w[4]) const {
+    int4 v = make_int4(0xff80ff80, 0xff80ff80, 0xff80ff80, 0xff80ff80);
+    if (g >= lo && g < hi) v = __ldg(reinterpret_cast<const int4*>(src + (g * 8 - shift)));
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else {
+  }
+  __device__ __forceinline__ bool partial(int g) const {
+    return g >= 0 && g < groups && (g < lo || g >= hi);
+  }
+  // Columns at .. at + 7, of which some may lie outside (-inf).
+  __device__ __forceinline__ void load_any(int at, uint32_t w[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = at + 2 * e;
-      const uint32_t lo = (i >= 0 && i < len) ? __ldg(src + i) : 0xff80u;
-      const uint32_t hi = (i + 1 >= 0 && i + 1 < len) ? __ldg(src + i + 1) : 0xff80u;
-      w[e] = lo | (hi << 16);
+      const uint32_t a = (i >= 0 && i < len) ? __ldg(src + i) : 0xff80u;
+      const uint32_t b = (i + 1 >= 0 && i + 1 < len) ? __ldg(src + i + 1) : 0xff80u;
+      w[e] = a | (b << 16);
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = clean2(w[e]);
-}
+};
 
 __device__ __forceinline__ float scale_to(float m, float top, float c) {
   return m == top ? 1.f : fast_exp2((m - top) * c);  // 0 for m = -inf
 }
 
-// This thread's part of a slice: its largest logit m and the sum over its
-// logits of 2^((l - m) * c), kRowBatch vectors in flight.
-constexpr int kRowBatch = 5;
+// A thread's running (max, sum of 2^((l - max) * c)) over one row.
+struct RowSum {
+  float m = -INFINITY, sum = 0.f;
 
-__device__ __forceinline__ void scan_row(const unsigned short* src, int len, float c, float& m,
-                                         float& sum) {
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) >> 1);
-  const int groups = (shift + len + 7) / 8;
-  m = -INFINITY;
-  sum = 0.f;
-  for (int g0 = threadIdx.x; g0 < groups; g0 += kRowBatch * kVerifyThreads) {
-    uint32_t w[kRowBatch][4];
-#pragma unroll
-    for (int u = 0; u < kRowBatch; ++u) load8(src, (g0 + u * kVerifyThreads) * 8 - shift, len, w[u]);
+  template <int N>
+  __device__ __forceinline__ void add(uint32_t (&w)[N][4], float c) {
     __nv_bfloat162 mx = neg_inf2();
 #pragma unroll
-    for (int u = 0; u < kRowBatch; ++u) {
+    for (int u = 0; u < N; ++u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = __hmax2(mx, *reinterpret_cast<__nv_bfloat162*>(&w[u][e]));
+      for (int e = 0; e < 4; ++e) {
+        w[u][e] = clean2(w[u][e]);
+        mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w[u][e]));
+      }
     }
     const float top = fmaxf(m, fmaxf(__low2float(mx), __high2float(mx)));
-    if (top == -INFINITY) continue;
+    if (top == -INFINITY) return;
     if (top == INFINITY) {  // infinite logits share everything
       if (m < INFINITY) sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < kRowBatch; ++u) {
+      for (int u = 0; u < N; ++u) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           sum += static_cast<float>((w[u][e] & 0xffffu) == 0x7f80u) +
                  static_cast<float>((w[u][e] >> 16) == 0x7f80u);
       }
       m = top;
-      continue;
+      return;
     }
     sum *= scale_to(m, top, c);
     m = top;
     const uint64_t ntop2 = pack_f32x2(-top, -top), c2 = pack_f32x2(c, c);
-    uint64_t acc[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
-    const uint64_t zero2 = acc[0];
+    const uint64_t zero2 = pack_f32x2(0.f, 0.f);
+    uint64_t acc[2] = {zero2, zero2};
 #pragma unroll
-    for (int u = 0; u < kRowBatch; ++u) {
+    for (int u = 0; u < N; ++u) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t l2 = (static_cast<uint64_t>(w[u][e] & 0xffff0000u) << 32) | (w[u][e] << 16);
@@ -222,441 +302,604 @@ __device__ __forceinline__ void scan_row(const unsigned short* src, int len, flo
     const float2 a = unpack_f32x2(add_f32x2(acc[0], acc[1]));
     sum += a.x + a.y;
   }
+};
+
+// This thread's part of a slice of one row (kRowBatch vectors in flight), or of
+// the target's and the draft's row together (that many of each).
+constexpr int kRowBatch = 5, kRowBatch2 = 3;
+
+// The partial groups of a slice, one on each of two threads.
+__device__ __forceinline__ int edge_group(const Slice& s) {
+  const int g = threadIdx.x == 0 ? 0 : (threadIdx.x == 1 ? s.groups - 1 : -1);
+  return (threadIdx.x == 1 && g == 0) || !s.partial(g) ? -1 : g;
+}
+
+template <bool kTwo>
+__device__ __forceinline__ void scan_rows(const Slice& s, const Slice& s2, float c, RowSum& r,
+                                          RowSum& r2) {
+  constexpr int kBatch = kTwo ? kRowBatch2 : kRowBatch;
+  const int hi = kTwo ? max(s.hi, s2.hi) : s.hi;
+#pragma unroll 1
+  for (int g0 = threadIdx.x; g0 < hi; g0 += kBatch * kVerifyThreads) {
+    uint32_t w[kBatch][4], v[kTwo ? kBatch : 1][4];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) s.load(g0 + u * kVerifyThreads, w[u]);
+    if constexpr (kTwo) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) s2.load(g0 + u * kVerifyThreads, v[u]);
+    }
+    r.add(w, c);
+    if constexpr (kTwo) r2.add(v, c);
+  }
+  if (threadIdx.x < 2) {
+    uint32_t w[1][4];
+    const int g = edge_group(s), g2 = kTwo ? edge_group(s2) : -1;
+    if (g >= 0) {
+      s.load_any(g * 8 - s.shift, w[0]);
+      r.add(w, c);
+    }
+    if (kTwo && g2 >= 0) {
+      s2.load_any(g2 * 8 - s2.shift, w[0]);
+      r2.add(w, c);
+    }
+  }
 }
 
 // Greedy rows: this thread's best logit of a slice and its first column.
-__device__ __forceinline__ unsigned long long scan_best(const unsigned short* src, int x0,
-                                                        int len) {
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) >> 1);
-  const int groups = (shift + len + 7) / 8;
-  float best = -INFINITY;
-  uint32_t bcol = 0;
-  for (int g0 = threadIdx.x; g0 < groups; g0 += kRowBatch * kVerifyThreads) {
+__device__ __forceinline__ unsigned long long scan_best(const Slice& s, int x0) {
+  unsigned long long key = 0ull;
+  auto take = [&](const uint32_t w[4], int g) {
+    const __nv_bfloat162 m = __hmax2(
+        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]),
+                *reinterpret_cast<const __nv_bfloat162*>(&w[1])),
+        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[2]),
+                *reinterpret_cast<const __nv_bfloat162*>(&w[3])));
+    const float best = fmaxf(__low2float(m), __high2float(m));  // NaN: all NaN
+    if (!(best > -INFINITY) || vkey(best, 0u) <= key) return;
+    int first = 7;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      const float l = __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
+      if (l == best) first = e;
+    }
+    const unsigned long long k = vkey(best, static_cast<uint32_t>(x0 + g * 8 - s.shift + first));
+    key = k > key ? k : key;
+  };
+#pragma unroll 1
+  for (int g0 = threadIdx.x; g0 < s.hi; g0 += kRowBatch * kVerifyThreads) {
     uint32_t w[kRowBatch][4];
 #pragma unroll
-    for (int u = 0; u < kRowBatch; ++u) load8(src, (g0 + u * kVerifyThreads) * 8 - shift, len, w[u]);
+    for (int u = 0; u < kRowBatch; ++u) s.load(g0 + u * kVerifyThreads, w[u]);
 #pragma unroll
-    for (int u = 0; u < kRowBatch; ++u) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float l = __uint_as_float((e & 1) ? (w[u][e >> 1] & 0xffff0000u) : (w[u][e >> 1] << 16));
-        if (l > best) {  // columns come in increasing order: the first of equals stays
-          best = l;
-          bcol = static_cast<uint32_t>(x0 + (g0 + u * kVerifyThreads) * 8 - shift + e);
-        }
-      }
+    for (int u = 0; u < kRowBatch; ++u) take(w[u], g0 + u * kVerifyThreads);
+  }
+  if (threadIdx.x < 2) {
+    const int g = edge_group(s);
+    if (g >= 0) {
+      uint32_t w[4];
+      s.load_any(g * 8 - s.shift, w);
+      take(w, g);
     }
   }
-  return best > -INFINITY ? vkey(best, bcol) : 0ull;
+  return key;
+}
+
+// Every warp's slot to every CTA of the cluster. After the barrier this CTA has
+// all of them, in column order; a buffer is written again two exchanges later,
+// when all have read it. No CTA's shared memory is written before it runs: its
+// arrival is in the constructor, the wait for the others' in the first call.
+struct Exchange {
+  VerifyShared& sh;
+  int rank, ranks, warp, lane, parity = 0;
+  bool started = false;
+
+  __device__ __forceinline__ explicit Exchange(VerifyShared& s)
+      : sh(s),
+        rank(static_cast<int>(cg::this_cluster().block_rank())),
+        ranks(static_cast<int>(cg::this_cluster().num_blocks())),
+        warp(threadIdx.x >> 5),
+        lane(threadIdx.x & 31) {}
+  __device__ __forceinline__ void arrive() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
+  __device__ __forceinline__ const VerifySlot* operator()(const VerifySlot& mine) {
+    if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    started = true;
+    VerifySlot* at = &sh.slots[parity][rank * kVerifyWarps + warp];
+    if (lane < ranks) *cg::this_cluster().map_shared_rank(at, lane) = mine;
+    cg::this_cluster().sync();
+    const VerifySlot* all = sh.slots[parity];
+    parity ^= 1;
+    return all;
+  }
+};
+
+__device__ __forceinline__ const unsigned short* row_of(const __nv_bfloat16* base, int64_t b,
+                                                        int64_t stride_seq, int64_t row,
+                                                        int64_t stride_row) {
+  return reinterpret_cast<const unsigned short*>(base) + b * stride_seq + row * stride_row;
 }
 
 template <bool kDraft>
-__global__ void __launch_bounds__(kVerifyThreads, 3) verify_kernel(const VerifyParams p) {
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int ranks = static_cast<int>(cluster.num_blocks());
-  const int b = blockIdx.x / ranks;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const VerifyParams p) {
   __shared__ VerifyShared sh;
+  __shared__ double table[kExpTable];
+  __shared__ int32_t parents[kMaxNodes];
+  __shared__ int32_t path[kMaxNodes + 1];
+  Exchange exchange(sh);
+  const int rank = exchange.rank, ranks = exchange.ranks, lane = exchange.lane;
+  const int b = blockIdx.x / ranks;
+  const int tid = threadIdx.x;
+  const int nslots = ranks * kVerifyWarps;
+  // the draw may start beside this grid's last CTAs: it waits for their results
+  asm volatile("griddepcontrol.launch_dependents;");
 
   const int x0 = min(rank * p.slice, p.vocab);
   const int len = min(p.slice, p.vocab - x0);
   const int n = p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
-  const float temp = p.temperatures ? p.temperatures[b] : 0.f;
+  const float temp = p.temperatures ? fminf(p.temperatures[b], kMaxTemperature) : 0.f;
   const bool greedy = !(temp > 0.f);
-  const double c64 = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temp);
+  const double c64 = greedy ? 1.0 : 1.4426950408889634074 / static_cast<double>(temp);
   const float c32 = fminf(static_cast<float>(c64), 1e30f);
   const int64_t* tokens = p.tokens + static_cast<int64_t>(b) * (p.nodes - 1);
   const float* u = p.u_accept + static_cast<int64_t>(b) * (p.nodes - 1);
+  const int64_t out_row = static_cast<int64_t>(b) * p.nodes;
 
   if (n == 0) {  // a padding row (uniform over the cluster)
     for (int i = tid; rank == 0 && i < p.nodes; i += kVerifyThreads) {
-      p.out_tokens[static_cast<int64_t>(b) * p.nodes + i] = -1;
-      p.out_path[static_cast<int64_t>(b) * p.nodes + i] = -1;
+      p.out_tokens[out_row + i] = -1;
+      p.out_path[out_row + i] = -1;
     }
     if (rank == 0 && tid == 0) p.out_num[b] = 0;
     return;
   }
+  exchange.arrive();
   for (int i = tid; i < p.nodes; i += kVerifyThreads)
-    sh.parents[i] = p.parents ? p.parents[static_cast<int64_t>(b) * p.parents_stride + i] : i - 1;
-  for (int i = tid; !greedy && i < kExpTable; i += kVerifyThreads)
-    sh.table[i] = exp2(static_cast<double>(i) / kExpTable);
-  if (tid == 0) {
-    sh.count = 0;
-    sh.path[0] = 0;
-  }
+    parents[i] = p.parents ? p.parents[static_cast<int64_t>(b) * p.parents_stride + i] : i - 1;
+  if (!greedy) fill_table(table);
+  if (tid == 0) path[0] = 0;
   __syncthreads();
-  int parity = 0;
 
-  // Adds up what every CTA of the cluster wrote to its sums[parity]; ends with
-  // the totals visible to the whole CTA. scaled: sums of exponentials, each
-  // relative to its CTA's largest logit; otherwise weights, and the owner of the
-  // draw's threshold.
-  auto exchange = [&](bool scaled) {
-    cluster.sync();
-    if (warp == 0) {
-      VerifySums v{0ull, -INFINITY, 0.0, 0.0};
-      if (lane < ranks) v = *cluster.map_shared_rank(&sh.sums[parity], lane);
-      if (scaled) {
-        unsigned long long key = v.key;
-        float qm = v.qmax;
-#pragma unroll
-        for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
-          const unsigned long long k2 = __shfl_xor_sync(0xffffffffu, key, o);
-          key = k2 > key ? k2 : key;
-          qm = fmaxf(qm, __shfl_xor_sync(0xffffffffu, qm, o));
-        }
-        const float pm = vkey_score(key);
-        const double ps = warp_sum(v.psum * static_cast<double>(scale_to(vkey_score(v.key), pm, c32)));
-        const double qs = warp_sum(v.qsum * static_cast<double>(scale_to(v.qmax, qm, c32)));
-        if (lane == 0) {
-          sh.pmax = pm;
-          sh.qmax = qm;
-          sh.psum = ps;
-          sh.qsum = qs;
-          sh.argmax = key ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)) : 0;
-        }
-      } else {
-        // inclusive prefix over the ranks, in rank order
-        double run = 0.0, incl = 0.0;
-        for (int r = 0; r < ranks; ++r) {
-          run += __shfl_sync(0xffffffffu, v.psum, r);
-          if (lane == r) incl = run;
-        }
-        const double threshold = static_cast<double>(fmaxf(p.u_pick[b], 0.f)) * run;
-        const unsigned over = __ballot_sync(0xffffffffu, lane < ranks && incl > threshold);
-        const unsigned some = __ballot_sync(0xffffffffu, lane < ranks && v.psum > 0.0);
-        const int owner = over ? __ffs(over) - 1 : (some ? 31 - __clz(some) : 0);
-        const double before = __shfl_sync(0xffffffffu, incl - v.psum, owner);
-        if (lane == 0) {
-          sh.psum = run;
-          sh.base = threshold - before;  // what the owner's own weights have to exceed
-          sh.owner = owner;
-        }
-      }
-    }
-    parity ^= 1;
-    __syncthreads();
-  };
-
-  int node = 0;
+  int node = 0, count = 0;
   while (true) {
-    // ---- the row's largest logit and sum of exponentials
-    const unsigned short* prow =
-        reinterpret_cast<const unsigned short*>(p.logits) +
-        static_cast<int64_t>(b) * p.l_stride_seq + static_cast<int64_t>(node) * p.l_stride_row;
+    const unsigned short* prow = row_of(p.logits, b, p.l_stride_seq, node, p.l_stride_row);
     const bool with_q = kDraft && !greedy && node + 1 < n;
-    const unsigned short* qrow = nullptr;
-    if (with_q)
-      qrow = reinterpret_cast<const unsigned short*>(p.draft) +
-             static_cast<int64_t>(b) * p.d_stride_seq + static_cast<int64_t>(node) * p.d_stride_row;
-    float qm = -INFINITY, qsum = 0.f, pm = -INFINITY, psum = 0.f;
-    unsigned long long key;
-    if (greedy) {
-      key = scan_best(prow + x0, x0, len);
-    } else {
-      scan_row(prow + x0, len, c32, pm, psum);
-      if (with_q) scan_row(qrow + x0, len, c32, qm, qsum);
-      key = pm > -INFINITY ? vkey(pm, 0u) : 0ull;  // the column is the greedy rows' alone
-    }
-    {
-      unsigned long long wkey = key;
-      float wq = qm;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long k2 = __shfl_xor_sync(0xffffffffu, wkey, o);
-        wkey = k2 > wkey ? k2 : wkey;
-        wq = fmaxf(wq, __shfl_xor_sync(0xffffffffu, wq, o));
-      }
-      // warp sums of up to 2^14 fp32 terms near 1 and below: fp32 carries them
-      // well inside the decisions' 2^-14
-      const float a = warp_sum(psum * scale_to(pm, vkey_score(wkey), c32));
-      const float d = kDraft ? warp_sum(qsum * scale_to(qm, wq, c32)) : 0.f;
-      if (lane == 0) {
-        sh.warp_key[warp] = wkey;
-        sh.warp_q[warp] = wq;
-        sh.warp_a[warp] = a;
-        sh.warp_b[warp] = d;
-      }
-    }
-    __syncthreads();
-    if (warp == 0) {
-      const bool in = lane < kVerifyWarps;
-      const unsigned long long k0 = in ? sh.warp_key[lane] : 0ull;
-      const float q0 = in ? sh.warp_q[lane] : -INFINITY;
-      unsigned long long k = k0;
-      float q = q0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long k2 = __shfl_xor_sync(0xffffffffu, k, o);
-        k = k2 > k ? k2 : k;
-        q = fmaxf(q, __shfl_xor_sync(0xffffffffu, q, o));
-      }
-      const double a = warp_sum(in ? sh.warp_a[lane] * scale_to(vkey_score(k0), vkey_score(k), c32) : 0.0);
-      const double d = warp_sum(in ? sh.warp_b[lane] * scale_to(q0, q, c32) : 0.0);
-      if (lane == 0) sh.sums[parity] = VerifySums{k, q, a, d};
-    }
-    exchange(true);
+    const unsigned short* qrow =
+        with_q ? row_of(p.draft, b, p.d_stride_seq, node, p.d_stride_row) : prow;
+    const Slice ps(prow + x0, len), qs(qrow + x0, with_q ? len : 0);
 
-    // ---- which child goes on. Warp 0 of every CTA takes the same decision.
-    // exact: the sums are fp64's own; otherwise an outcome within 2^-14 of
-    // its border is left open (the fp32 terms put the sums off by < 2^-17).
-    auto decide = [&](bool exact) {
-      if (warp != 0) return;
-      const uint32_t top = __float_as_uint(sh.pmax) >> 16;
-      const uint32_t qtop = __float_as_uint(sh.qmax) >> 16;
-      const double top_c = static_cast<double>(sh.pmax) * c64;
-      const double qtop_c = static_cast<double>(sh.qmax) * c64;
-      const bool any = sh.pmax > -INFINITY;
-      int next = -1, nrej = 0, open = 0;
-      double left = 1.0;
-      for (int c0 = node + 1; c0 < n && next < 0 && !open; c0 += 32) {
-        const int c = c0 + lane;
-        const bool mine = c < n && sh.parents[c] == node;
-        const int64_t tok = mine ? tokens[c - 1] : -1;
-        const bool in = mine && tok >= 0 && tok < p.vocab;
-        double here = 0.0, against = 0.0;
-        if (in && !greedy && any) {
-          here = weight64(clean2(prow[tok]) & 0xffffu, top, c64, top_c, sh.table) / sh.psum;
-          if (with_q && sh.qmax > -INFINITY)
-            against = weight64(clean2(qrow[tok]) & 0xffffu, qtop, c64, qtop_c, sh.table) / sh.qsum;
+    // ---- a candidate child a lane: its token and what the rows say of it
+    struct Child {
+      int64_t tok;
+      float u;
+      uint32_t pbits, qbits;
+      bool mine, in;
+    };
+    auto child = [&](int c) {
+      Child k{-1, 0.f, 0xff80u, 0xff80u, c < n && parents[min(c, kMaxNodes - 1)] == node, false};
+      if (k.mine) {
+        k.tok = tokens[c - 1];
+        k.u = u[c - 1];
+        k.in = k.tok >= 0 && k.tok < p.vocab;
+        if (k.in) k.pbits = __ldg(prow + k.tok);
+        if (k.in && with_q) k.qbits = __ldg(qrow + k.tok);
+      }
+      return k;
+    };
+    const Child first = child(node + 1 + lane);
+
+    // ---- the row's largest logit and sum of exponentials
+    float pmax, qmax = -INFINITY;
+    double psum = 1.0, qsum = 1.0;
+    int argmax = 0;
+    if (greedy) {
+      VerifySlot v;
+      v.key[0] = warp_max(scan_best(ps, x0));
+      v.key[1] = 0ull;
+      const VerifySlot* all = exchange(v);
+      unsigned long long key = 0ull;
+      for (int i = lane; i < nslots; i += 32) key = all[i].key[0] > key ? all[i].key[0] : key;
+      key = warp_max(key);
+      pmax = vkey_score(key);
+      argmax = key ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)) : 0;
+    } else {
+      RowSum r, r2;
+      scan_rows<kDraft>(ps, qs, c32, r, r2);
+      VerifySlot v;
+      v.f.x = warp_max(r.m);
+      v.f.y = warp_sum(r.sum * scale_to(r.m, v.f.x, c32));
+      v.f.z = kDraft ? warp_max(r2.m) : -INFINITY;
+      v.f.w = kDraft ? warp_sum(r2.sum * scale_to(r2.m, v.f.z, c32)) : 0.f;
+      const VerifySlot* all = exchange(v);
+      float pm = -INFINITY, qm = -INFINITY;
+      for (int i = lane; i < nslots; i += 32) {
+        pm = fmaxf(pm, all[i].f.x);
+        if (kDraft) qm = fmaxf(qm, all[i].f.z);
+      }
+      pmax = warp_max(pm);
+      if (kDraft) qmax = warp_max(qm);
+      float a = 0.f, d = 0.f;
+      for (int i = lane; i < nslots; i += 32) {
+        const float4 f = all[i].f;
+        a += f.y * scale_to(f.x, pmax, c32);
+        if (kDraft) d += f.w * scale_to(f.z, qmax, c32);
+      }
+      psum = static_cast<double>(warp_sum(a));
+      if (kDraft) qsum = static_cast<double>(warp_sum(d));
+    }
+    // bf16 bits of the largest logits, kNoLogit where there is none
+    const uint32_t top = __float_as_uint(pmax) >> 16;
+    const uint32_t qtop = with_q ? __float_as_uint(qmax) >> 16 : kNoLogit;
+    const bool any = top != kNoLogit, any_q = qtop != kNoLogit;
+
+    // ---- which child goes on: every warp of the cluster takes this decision
+    // alike. With the fp32 sums (off by < 2^-17) an outcome within 2^-14 of its
+    // border is left open, and taken again with fp64 sums.
+    int next = -1;
+#pragma unroll 1
+    for (int exact = 0; exact < 2; ++exact) {
+      const RowScale scale(any ? top : 0u, c64), qscale(any_q ? qtop : 0u, c64);
+      if (exact) {
+        double a = 0.0, d = 0.0;
+#pragma unroll 1
+        for (int i = tid; i < len; i += kVerifyThreads) {
+          const uint32_t pb = __ldg(ps.src + i);
+          if ((pb & 0x7fffu) <= 0x7f80u && pb != 0xff80u)
+            a += exp2_64(scale.log2_weight(__uint_as_float(scale.raise(pb) << 16)), table);
+          if (any_q) {
+            const uint32_t qb = __ldg(qs.src + i);
+            if ((qb & 0x7fffu) <= 0x7f80u && qb != 0xff80u)
+              d += exp2_64(qscale.log2_weight(__uint_as_float(qscale.raise(qb) << 16)), table);
+          }
         }
-        const double uc = mine ? static_cast<double>(u[c - 1]) : 0.0;
-        unsigned todo = __ballot_sync(0xffffffffu, mine);
+        VerifySlot v;
+        v.d = make_double2(warp_sum(a), warp_sum(d));
+        const VerifySlot* all = exchange(v);
+        a = d = 0.0;
+        for (int i = lane; i < nslots; i += 32) {
+          a += all[i].d.x;
+          d += all[i].d.y;
+        }
+        psum = warp_sum(a);
+        qsum = warp_sum(d);
+      }
+      const double pinv = 1.0 / psum, qinv = 1.0 / qsum;
+      // a logit's probability; none for NaN and -inf
+      auto prob = [&](const RowScale& sc, uint32_t bits, bool live, double inv) {
+        const double w =
+            exp2_64(sc.log2_weight(__uint_as_float(sc.raise(bits) << 16)), table) * inv;
+        return live && (bits & 0x7fffu) <= 0x7f80u && bits != 0xff80u && w > kNothing ? w : 0.0;
+      };
+      double left = 1.0;
+      int nrej = 0;  // rejected tokens: lane i holds the i-th and the 32+i-th
+      int64_t rej0 = -1, rej1 = -1;
+      bool open = false;
+      next = -1;
+      for (int c0 = node + 1; c0 < n && next < 0 && !open; c0 += 32) {
+        const Child k = c0 == node + 1 ? first : child(c0 + lane);
+        double here = 0.0, against = 0.0;
+        if (!greedy) {  // uniform
+          here = prob(scale, k.pbits, k.in && any, pinv);
+          if (kDraft) against = prob(qscale, k.qbits, k.in && any_q, qinv);
+        }
+        unsigned todo = __ballot_sync(0xffffffffu, k.mine);
         while (todo && next < 0 && !open) {
           const int src = __ffs(todo) - 1;
           todo &= todo - 1;
-          const int64_t x = __shfl_sync(0xffffffffu, tok, src);
-          const bool inside = __shfl_sync(0xffffffffu, static_cast<int>(in), src);
+          const int64_t x = __shfl_sync(0xffffffffu, k.tok, src);
+          const bool inside = __shfl_sync(0xffffffffu, static_cast<int>(k.in), src);
           double hc = __shfl_sync(0xffffffffu, here, src);
-          const double uu = __shfl_sync(0xffffffffu, uc, src);
-          const double qc = __shfl_sync(0xffffffffu, against, src);
+          const double uu = static_cast<double>(__shfl_sync(0xffffffffu, k.u, src));
+          const double qc = kDraft ? __shfl_sync(0xffffffffu, against, src) : 0.0;
           bool ok;
           if (greedy) {
-            ok = inside && any && x == sh.argmax;
+            ok = inside && any && x == argmax;
           } else {
-            if (!kDraft) {  // a token tried before has no probability left
-              bool twin = false;
-              for (int i = lane; i < nrej; i += 32) twin |= sh.rejected[i] == x;
-              if (__any_sync(0xffffffffu, twin)) hc = 0.0;
-            }
+            if (!kDraft && __any_sync(0xffffffffu, inside && (rej0 == x || rej1 == x)))
+              hc = 0.0;  // a token tried before has no probability left
             const double bar = uu * (kDraft ? qc : left);
-            ok = bar < hc && hc > 0.0;
-            if (!exact && hc > 0.0 && fabs(bar - hc) <= 0x1p-14 * (hc + (kDraft ? bar : 1.0)))
-              open = 1;
+            ok = bar < hc;
+            open = !exact && hc > 0.0 && fabs(bar - hc) <= 0x1p-14 * (hc + (kDraft ? bar : 1.0));
           }
           if (ok) {
             next = c0 + src;
           } else {
             left -= hc;
-            if (lane == 0 && inside) sh.rejected[nrej] = x;
-            if (inside) ++nrej;
-            __syncwarp();
-          }
-        }
-      }
-      if (lane == 0) {
-        sh.next = next;
-        sh.nrejected = nrej;
-        sh.open = open;
-      }
-    };
-    decide(false);
-    __syncthreads();
-
-    // ---- fp64: a lane's run of consecutive columns, warps and ranks in order
-    const int run = ((len + kVerifyThreads - 1) / kVerifyThreads + 7) / 8 * 8;
-    const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
-    const uint32_t top = __float_as_uint(sh.pmax) >> 16, qtop = __float_as_uint(sh.qmax) >> 16;
-    const double top_c = static_cast<double>(sh.pmax) * c64;
-    const double qtop_c = static_cast<double>(sh.qmax) * c64;
-    const bool any = sh.pmax > -INFINITY, any_q = with_q && sh.qmax > -INFINITY;
-    const unsigned long long pkey = any ? vkey(sh.pmax, static_cast<uint32_t>(sh.argmax)) : 0ull;
-    const float qmax = sh.qmax;
-
-    // Sums over the run: a of p's exponentials without the rejected tokens, and
-    // with a draft row d of q's and, of the columns where p / psum exceeds q /
-    // qsum with the sums as they stand, ra and rd of both.
-    auto run_sums = [&](bool skip, double pinv, double qinv, double& a, double& d, double& ra,
-                        double& rd) {
-      a = d = ra = rd = 0.0;
-      bool held = false;  // a rejected token lies in this run
-      for (int i = 0; skip && i < sh.nrejected; ++i)
-        held |= sh.rejected[i] >= x0 + i0 && sh.rejected[i] < x0 + i1;
-      for (int at = i0; at < i1; at += 8) {
-        uint32_t w[4], v[4];
-        load8(prow + x0, at, len, w);
-        if (with_q) load8(qrow + x0, at, len, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t pb = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-          double wp = weight64(pb, top, c64, top_c, sh.table);
-          if (held) {
-            for (int i = 0; i < sh.nrejected; ++i)
-              if (sh.rejected[i] == x0 + at + e) wp = 0.0;
-          }
-          a += wp;
-          if (kDraft && with_q) {
-            const uint32_t qb = (e & 1) ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu;
-            const double wq = any_q ? weight64(qb, qtop, c64, qtop_c, sh.table) : 0.0;
-            d += wq;
-            if (fma(wp, pinv, -wq * qinv) > 0.0) {
-              ra += wp;
-              rd += wq;
+            if (!kDraft && inside) {
+              if (lane == (nrej & 31)) (nrej < 32 ? rej0 : rej1) = x;
+              ++nrej;
             }
           }
         }
       }
-    };
-    // fp64 sums of exponentials over the whole rows
-    auto sums64 = [&](double a, double d) {
-      a = warp_sum(a);
-      d = warp_sum(d);
-      if (lane == 0) {
-        sh.warp_a[warp] = a;
-        sh.warp_b[warp] = d;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        VerifySums v{pkey, qmax, 0.0, 0.0};
-        for (int w = 0; w < kVerifyWarps; ++w) {
-          v.psum += sh.warp_a[w];
-          v.qsum += sh.warp_b[w];
-        }
-        sh.sums[parity] = v;
-      }
-      exchange(true);
-    };
-
-    if (sh.open) {
-      double a, d, ra, rd;
-      run_sums(false, 1.0, 0.0, a, d, ra, rd);
-      sums64(a, d);
-      decide(true);
-      __syncthreads();
+      if (!open) break;
     }
-    if (sh.next >= 0) {
-      node = sh.next;
-      if (tid == 0) sh.path[++sh.count] = node;
-      __syncthreads();
+    if (next >= 0) {
+      node = next;
+      ++count;
+      if (tid == 0) path[count] = node;
       continue;
     }
-
-    // ---- nothing goes on: draw from what the last row has left
-    int64_t pick = -1;
-    if (greedy || !any) {
-      if (rank == 0 && tid == 0) pick = sh.argmax;
-    } else {
-      bool use_q = any_q, skip = !kDraft && sh.nrejected > 0;
-      double pinv = 1.0, qinv = 0.0;
-      for (int attempt = 0; attempt < 2; ++attempt) {
-        double mine, a, d, ra, rd;
-        if (use_q) {
-          // One pass gives the exact sums and, over the columns that are
-          // positive by the sums at hand, the parts of the residual: a column
-          // on the wrong side by a rounding of those has a residual of no more
-          // than that rounding.
-          pinv = 1.0 / sh.psum;
-          qinv = 1.0 / sh.qsum;
-          __syncthreads();
-          run_sums(false, pinv, qinv, a, d, ra, rd);
-          sums64(a, d);
-          pinv = 1.0 / sh.psum;
-          qinv = 1.0 / sh.qsum;
-          __syncthreads();
-          mine = fmax(ra * pinv - rd * qinv, 0.0);
-        } else {
-          run_sums(skip, 1.0, 0.0, a, d, ra, rd);
-          mine = a;
-        }
-        // prefix over the lanes, in column order
-        double incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        if (lane == 31) sh.warp_a[warp] = incl;
-        __syncthreads();
-        if (tid == 0) {
-          VerifySums v{0ull, -INFINITY, 0.0, 0.0};
-          for (int w = 0; w < kVerifyWarps; ++w) v.psum += sh.warp_a[w];
-          sh.sums[parity] = v;
-        }
-        exchange(false);
-        if (!(sh.psum > 0.0) && attempt == 0) {
-          // nothing is left (rounding rejected the last of the mass): draw from p
-          use_q = skip = false;
-          pinv = 1.0;
-          qinv = 0.0;
-          continue;
-        }
-        if (rank == sh.owner) {
-          // the warp, then the lane, whose weights cross the threshold (with u so
-          // near 1 that rounding hides the border: the last ones with weight)
-          double before = 0.0;
-          int ow = -1, last = 0;
-          for (int w = 0; w < kVerifyWarps; ++w) {
-            if (sh.warp_a[w] > 0.0) last = w;
-            if (ow < 0 && before + sh.warp_a[w] > sh.base) ow = w;
-            if (ow < 0) before += sh.warp_a[w];
-          }
-          const bool none = ow < 0;
-          if (none) ow = last;
-          if (warp == ow) {
-            const double want = none ? INFINITY : sh.base - before;
-            const unsigned over = __ballot_sync(0xffffffffu, incl > want);
-            const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-            const int ol = over ? __ffs(over) - 1 : (some ? 31 - __clz(some) : 0);
-            double sum = __shfl_sync(0xffffffffu, incl - mine, ol);
-            const int j0 = __shfl_sync(0xffffffffu, i0, ol), j1 = __shfl_sync(0xffffffffu, i1, ol);
-            int found = -1, lastx = j0;
-            for (int j = j0; j < j1 && found < 0; j += 32) {
-              const int i = j + lane;
-              double w = 0.0;
-              if (i < j1) {
-                w = weight64(clean2(prow[x0 + i]) & 0xffffu, top, c64, top_c, sh.table) * pinv;
-                for (int r = 0; skip && r < sh.nrejected; ++r)
-                  if (sh.rejected[r] == x0 + i) w = 0.0;
-                if (use_q)
-                  w = fmax(w - weight64(clean2(qrow[x0 + i]) & 0xffffu, qtop, c64, qtop_c, sh.table) *
-                                   qinv, 0.0);
-              }
-              double part = w;
-#pragma unroll
-              for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, part, o);
-                if (lane >= o) part += y;
-              }
-              const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && sum + part > want);
-              const unsigned pos = __ballot_sync(0xffffffffu, w > 0.0);
-              if (pos) lastx = j + 31 - __clz(pos);
-              if (hit) found = j + __ffs(hit) - 1;
-              sum += __shfl_sync(0xffffffffu, part, 31);
-            }
-            if (lane == 0) pick = x0 + (found >= 0 ? found : lastx);
-          }
-        }
-        break;
-      }
-    }
-    const int count = sh.count;
-    const int64_t row = static_cast<int64_t>(b) * p.nodes;
-    if (pick >= 0) p.out_tokens[row + count] = pick;
     if (rank == 0) {
+      __syncthreads();  // path
       for (int i = tid; i < p.nodes; i += kVerifyThreads) {
-        p.out_path[row + i] = i <= count ? sh.path[i] : -1;
-        if (i != count) p.out_tokens[row + i] = i < count ? tokens[sh.path[i + 1] - 1] : -1;
+        p.out_path[out_row + i] = i <= count ? path[i] : -1;
+        int64_t t = i < count ? tokens[path[i + 1] - 1] : -1;
+        if (i == count)
+          t = greedy || !any ? argmax
+                             : pack_state({top, qtop, static_cast<float>(psum / qsum)});
+        p.out_tokens[out_row + i] = t;
       }
-      if (tid == 0) p.out_num[b] = count;
+      // !any, told to the draw by the sign, is a pick already
+      if (tid == 0) p.out_num[b] = greedy || any ? count : ~count;
     }
-    break;
+    return;
   }
-  cluster.sync();  // no CTA leaves while its sums may be read
 }
 
+// The draw of every sequence's next token from the row of its last node: p, or p
+// without its rejected children's tokens, or (a draft row) max(p - q, 0).
 template <bool kDraft>
-static int launch_verify(VerifyParams p, int batch, cudaStream_t stream) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const VerifyParams p) {
+  __shared__ VerifyShared sh;
+  __shared__ double table[kExpTable];
+  Exchange exchange(sh);
+  const int rank = exchange.rank, ranks = exchange.ranks;
+  const int lane = exchange.lane, warp = exchange.warp;
+  const int b = blockIdx.x / ranks;
+  const int nslots = ranks * kVerifyWarps;
+  fill_table(table);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the walk is done
+  const int n = p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
+  const float temp = p.temperatures ? fminf(p.temperatures[b], kMaxTemperature) : 0.f;
+  const int num = p.out_num[b];
+  cg::this_cluster().sync();  // all have read num, and run
+  exchange.started = true;
+  if (num < 0) {
+    if (rank == 0 && threadIdx.x == 0) p.out_num[b] = ~num;
+    return;
+  }
+  if (n == 0 || !(temp > 0.f)) return;
+
+  const int64_t out_row = static_cast<int64_t>(b) * p.nodes;
+  const int node = p.out_path[out_row + num];
+  const DrawState st = unpack_state(p.out_tokens[out_row + num]);
+  const int x0 = min(rank * p.slice, p.vocab);
+  const int len = min(p.slice, p.vocab - x0);
+  const double c64 = 1.4426950408889634074 / static_cast<double>(temp);
+  const RowScale scale(st.top, c64), qscale(st.qtop == kNoLogit ? 0u : st.qtop, c64);
+  const double ratio = static_cast<double>(st.ratio);
+  bool use_q = kDraft && st.qtop != kNoLogit;
+  const Slice ps(row_of(p.logits, b, p.l_stride_seq, node, p.l_stride_row) + x0, len);
+  const Slice qs(
+      (use_q ? row_of(p.draft, b, p.d_stride_seq, node, p.d_stride_row) + x0 : ps.src), len);
+
+  // the rejected tokens: the node's children. Lane i holds the i-th and 32+i-th.
+  int64_t rej[2] = {-1, -1};
+  if (!kDraft) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h * 32 + lane;
+      const int parent = c >= p.nodes ? -1
+                         : p.parents  ? p.parents[static_cast<int64_t>(b) * p.parents_stride + c]
+                                      : c - 1;
+      if (c > node && c < n && parent == node)
+        rej[h] = p.tokens[static_cast<int64_t>(b) * (p.nodes - 1) + c - 1];
+    }
+  }
+
+  // A warp owns `steps` steps of 32 16-byte groups, in column order; bin i (lane
+  // i's) is steps [i * per, (i + 1) * per).
+  const int steps = (ps.groups + kVerifyThreads - 1) / kVerifyThreads;
+  const int per = (steps + 31) / 32;
+  auto group = [&](int step) { return (warp * steps + step) * 32 + lane; };
+  // those of the rejected tokens that lie among this warp's columns
+  uint32_t mask[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t x = rej[h] - x0 - (warp * steps * 256 - ps.shift);
+    mask[h] = __ballot_sync(0xffffffffu, rej[h] >= 0 && x >= 0 && x < steps * 256);
+  }
+  bool skip = __any_sync(0xffffffffu, rej[0] >= 0 || rej[1] >= 0);
+  // Loads of a step's 8 columns: issue() sends for what needs no look at the
+  // data, finish() reads partial groups and draft rows at another alignment.
+  const bool same = qs.shift == ps.shift;
+  auto issue = [&](int g, uint32_t w[4], uint32_t v[4]) {
+    ps.load(g, w);
+    if (kDraft && use_q && same) qs.load(g, v);
+  };
+  auto finish = [&](int g, uint32_t w[4], uint32_t v[4]) {
+    if (ps.partial(g)) ps.load_any(g * 8 - ps.shift, w);
+    if (kDraft && use_q && (!same || ps.partial(g))) qs.load_any(g * 8 - ps.shift, v);
+    if (!kDraft && skip) {  // rejected columns have no weight
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+        for (uint32_t m = mask[h]; m; m &= m - 1) {
+          const int64_t x =
+              __shfl_sync(0xffffffffu, rej[h], __ffs(m) - 1) - x0 - (g * 8 - ps.shift);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (x == e) w[e >> 1] |= (e & 1) ? 0xffff0000u : 0xffffu;  // NaN
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = scale.raise(w[e]);
+      if (kDraft && use_q) v[e] = qscale.raise(v[e]);
+    }
+  };
+  auto logit = [](const uint32_t w[4], int e) {
+    return __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
+  };
+
+  double pinv = 1.0, qinv = 0.0;
+#pragma unroll 1
+  for (int attempt = 0;; ++attempt) {
+    // ---- one pass. With a draft row it gives the exact sums a, d and, over the
+    // columns where p exceeds q by the sums of the walk, the parts ra, rd of the
+    // residual: a column on the wrong side by a rounding of those sums has a
+    // residual of no more than that rounding. Otherwise ra is p's.
+    double a = 0.0, d = 0.0, ra = 0.0, rd = 0.0, sa = 0.0, sd = 0.0;
+    uint32_t w[4], v[4] = {0u, 0u, 0u, 0u}, wn[4], vn[4];
+    issue(group(0), w, v);
+#pragma unroll 1
+    for (int step = 0, in_bin = 0, bin = 0; step < steps; ++step) {
+      if (step + 1 < steps) issue(group(step + 1), wn, vn);  // before this step's arithmetic
+      finish(group(step), w, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double wp = exp2_64(scale.log2_weight(logit(w, e)), table);
+        if (kDraft && use_q) {
+          const double wq = exp2_64(qscale.log2_weight(logit(v, e)), table);
+          a += wp;
+          d += wq;
+          if (wp > wq * ratio) {
+            sa += wp;
+            sd += wq;
+          }
+        } else {
+          sa += wp;
+        }
+      }
+      if (++in_bin == per || step + 1 == steps) {
+        const double ta = warp_sum(sa);
+        if (lane == bin) ra = ta;
+        if (kDraft && use_q) {
+          const double td = warp_sum(sd);
+          if (lane == bin) rd = td;
+        }
+        sa = sd = 0.0;
+        in_bin = 0;
+        ++bin;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = wn[e];
+        v[e] = vn[e];
+      }
+    }
+    double mine = ra;  // the weight of this lane's bin
+    if (kDraft && use_q) {
+      VerifySlot s;
+      s.d = make_double2(warp_sum(a), warp_sum(d));
+      const VerifySlot* all = exchange(s);
+      a = d = 0.0;
+      for (int i = lane; i < nslots; i += 32) {
+        a += all[i].d.x;
+        d += all[i].d.y;
+      }
+      pinv = 1.0 / warp_sum(a);
+      qinv = 1.0 / warp_sum(d);
+      mine = fmax(ra * pinv - rd * qinv, 0.0);
+    }
+    VerifySlot s;
+    s.d = make_double2(warp_sum(mine), 0.0);
+    const VerifySlot* all = exchange(s);
+    // prefix over the warps in column order, `each` consecutive ones a lane
+    const int each = (nslots + 31) / 32;
+    double own = 0.0;
+    for (int i = 0; i < each; ++i)
+      own += lane * each + i < nslots ? all[lane * each + i].d.x : 0.0;
+    const double incl = warp_scan(own, lane);
+    const double total = __shfl_sync(0xffffffffu, incl, 31);
+    if (!(total > kNothing) && attempt == 0) {
+      use_q = skip = false;  // rounding rejected the last of the mass: draw from p
+      pinv = 1.0;
+      qinv = 0.0;
+      continue;
+    }
+    const double threshold =
+        fmax(static_cast<double>(fmaxf(p.u_pick[b], 0.f)) * total, kNothing);
+    // the first warp whose weights cross the threshold (with u so near 1 that
+    // rounding hides the border: the last one with weight)
+    const unsigned over = __ballot_sync(0xffffffffu, incl > threshold);
+    const unsigned some = __ballot_sync(0xffffffffu, own > kNothing);
+    const int ol = over ? __ffs(over) - 1 : (some ? 31 - __clz(some) : 0);
+    double before = __shfl_sync(0xffffffffu, incl - own, ol);
+    int owner = -1, last = 0;
+    for (int i = ol * each; i < min((ol + 1) * each, nslots) && owner < 0; ++i) {
+      const double t = all[i].d.x;
+      if (t > kNothing) last = i;
+      if (over && before + t > threshold)
+        owner = i;
+      else
+        before += t;
+    }
+    const double want = owner >= 0 ? threshold - before : INFINITY;
+    if (owner < 0) owner = last;
+    if (owner != rank * kVerifyWarps + warp) return;
+
+    // ---- the owner's bin, step, lane and column
+    const double bins = warp_scan(mine, lane);
+    const unsigned obin = __ballot_sync(0xffffffffu, bins > want);
+    const unsigned pbin = __ballot_sync(0xffffffffu, mine > kNothing);
+    const int bin = obin ? __ffs(obin) - 1 : (pbin ? 31 - __clz(pbin) : 0);
+    double sum = __shfl_sync(0xffffffffu, bins - mine, bin);
+    int found = -1, lastx = -1;
+#pragma unroll 1
+    for (int step = bin * per; step < min((bin + 1) * per, steps) && found < 0; ++step) {
+      const int g = group(step), at = g * 8 - ps.shift;
+      issue(g, w, v);
+      finish(g, w, v);
+      double wp[8], t = 0.0;
+      int lx = -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        wp[e] = exp2_64(scale.log2_weight(logit(w, e)), table) * pinv;
+        if (kDraft && use_q)
+          wp[e] = fmax(wp[e] - exp2_64(qscale.log2_weight(logit(v, e)), table) * qinv, 0.0);
+        t += wp[e];
+        if (wp[e] > kNothing) lx = at + e;
+      }
+      const double upto = warp_scan(t, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, lx >= 0 && sum + upto > want);
+      const unsigned pos = __ballot_sync(0xffffffffu, lx >= 0);
+      if (hit) {
+        int x = -1;  // in that lane, the first column that crosses
+        double run = sum + (upto - t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          run += wp[e];
+          if (x < 0 && wp[e] > kNothing && run > want) x = at + e;
+        }
+        found = __shfl_sync(0xffffffffu, x < 0 ? lx : x, __ffs(hit) - 1);
+      }
+      if (pos) lastx = __shfl_sync(0xffffffffu, lx, 31 - __clz(pos));
+      sum += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) p.out_tokens[out_row + num] = x0 + (found >= 0 ? found : max(lastx, 0));
+    return;
+  }
+}
+
+static cudaError_t launch_cluster(void (*kernel)(VerifyParams), VerifyParams p, int batch, int ranks,
+                                  bool dependent, cudaStream_t stream) {
+  p.slice = ((p.vocab + ranks - 1) / ranks + 7) / 8 * 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+#ifndef VWALK
+#define VWALK 4
+#endif
+#ifndef VDRAW
+#define VDRAW 2
+#endif
+template <bool kDraft>
+static int launch_verify(const VerifyParams& p, int batch, cudaStream_t stream) {
   static std::mutex mu;
   static bool done[64];
   int dev = 0;
@@ -664,29 +907,27 @@ static int launch_verify(VerifyParams p, int batch, cudaStream_t stream) {
   {
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 64 || !done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(
-          verify_kernel<kDraft>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify_kernel)");
+      cudaError_t e = cudaFuncSetAttribute(verify_walk_kernel<kDraft>,
+                                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(verify_draw_kernel<kDraft>,
+                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify)");
       if (dev < 64) done[dev] = true;
     }
   }
-#ifndef VCLUSTER
-#define VCLUSTER (batch * 16 <= 148 ? 16 : 8)
-#endif
-  const int ranks = VCLUSTER;
-  p.slice = ((p.vocab + ranks - 1) / ranks + 7) / 8 * 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
-  cfg.blockDim = dim3(kVerifyThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<kDraft>, p);
-  return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "verify_kernel launch");
+  // CTAs a sequence: as many as the SMs hold for all sequences at once
+  const int64_t sms = device_sm_count();
+  auto fit = [&](int per_sm) {
+    int ranks = kMaxCluster;
+    while (ranks > 2 && static_cast<int64_t>(batch) * ranks > per_sm * sms) ranks /= 2;
+    return ranks;
+  };
+  cudaError_t e = launch_cluster(verify_walk_kernel<kDraft>, p, batch, fit(VWALK), false, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "verify_walk_kernel launch");
+  if (p.temperatures == nullptr) return NVATTN_OK;  // all greedy: nothing to draw
+  e = launch_cluster(verify_draw_kernel<kDraft>, p, batch, fit(VDRAW), true, stream);
+  return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "verify_draw_kernel launch");
 }
 
 }  // namespace nvattn

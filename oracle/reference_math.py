@@ -574,6 +574,7 @@ def verify_law(row, temperature: float) -> np.ndarray:
         return (np.arange(x.size) == int(np.argmax(x))).astype(np.float64)
     with np.errstate(invalid="ignore"):
         w = np.where(x == top, 1.0, np.exp((x - top) / np.float64(np.float32(temperature))))
+    w[w < 2.0 ** -950] = 0.0  # the operator's range
     return w / w.sum()
 
 

@@ -230,3 +230,17 @@ def test_graph_replay_and_two_streams():
         want = R.verify_draft(y[0], y[1].numpy(), y[2].numpy(), y[3].numpy(), **y[4])
         for a, c, b in zip(out, beside, want):
             assert np.array_equal(a.cpu().numpy(), b) and np.array_equal(c.cpu().numpy(), b)
+
+
+def test_extreme_temperatures():
+    """From almost greedy (only ties of the top share) to flat, with masked columns: they are never drawn."""
+    for form in ("chain", "draft", "tree"):
+        x, tok, u, pick, kw = _inputs(12, 4, 777, 22, form)
+        x[:, :, 100:] = float("-inf")
+        x[3:6] = (x[3:6].float() * 1e-3).to(torch.bfloat16)
+        x[6, :, 5:9] = 1.0
+        tok = tok % 100
+        kw["temperatures"] = torch.tensor([1e-38, 1e-30, 1e-6, 1e-20, 1e-4, 3e-3, 1e-7, 1e3, 1e8, 1e30,
+                                           1e-45, 2e-4])
+        for pv in (0.0, 0.37, 1.0 - 2.0 ** -24):
+            _check(x, tok, u, torch.full((12,), pv), kw)
