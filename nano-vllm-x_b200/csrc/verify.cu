@@ -19,13 +19,14 @@
 //
 // Two kernels. The walk reads only the rows on the path: one cluster of CTAs per
 // sequence, a CTA per slice of the columns. A row costs one pass with one MUFU
-// exponential and about four other instructions a logit (each thread sums
+// exponential and about three other instructions a logit (each thread sums
 // against its own maximum) and one cluster barrier: every warp writes its sums
 // into the shared memory of all CTAs, and after the barrier every warp adds the
-// same numbers up and takes the same decision, with nothing to broadcast. It is
-// kept to 64 registers and short code: rows are a chain, so what hides their
-// latency is other sequences on the same SM. The draw then goes over each
-// sequence's last row, all sequences at once.
+// same numbers up and takes the same decision, with nothing to broadcast. Rows
+// are a chain, bound by latency (about 5 us a node): the next node's rows are
+// sent for to L2 before it is accepted, and the code of a step is kept short
+// (it once overran the instruction cache at twice the time). The draw then goes
+// over each sequence's last row, all sequences at once.
 //
 // The answers are tokens, so sums that decide between neighbours are kept in
 // 64 bits: the draw's cumulative weights always (with 151,936 weights of which
@@ -71,6 +72,7 @@ struct VerifyParams {
   const float* temperatures;   // null: greedy
   const int32_t* num_nodes;    // null: all
   int32_t nodes, vocab, slice;
+  int32_t ahead;  // the walk sends for the first child's rows before it is accepted
   int64_t* out_tokens;
   int32_t* out_path;
   int32_t* out_num;
@@ -138,7 +140,7 @@ struct RowScale {
                            : (top_bits & 0x8000u)     ? top_bits + 1u
                                                       : top_bits - 1u;
     const double gap = static_cast<double>(top) - static_cast<double>(__uint_as_float(below << 16));
-    c = inf ? 1.0 : fmin(c64, 2000.0 / gap);
+    c = inf ? 1.0 : (c64 * gap > 2000.0 ? 2000.0 / gap : c64);
     top_c = inf ? 0.0 : static_cast<double>(top) * c;
   }
   // NaN and -inf become the lowest bf16.
@@ -237,6 +239,14 @@ struct Slice {
     if (g >= lo && g < hi) v = __ldg(reinterpret_cast<const int4*>(src + (g * 8 - shift)));
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
+  // Sends the whole groups to L2, one thread's instruction: the registers hold a
+  // few vectors a thread in flight, this holds the slice.
+  __device__ __forceinline__ void prefetch() const {
+    if (hi > lo)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + (lo * 8 - shift)),
+                   "r"((hi - lo) * 16)
+                   : "memory");
+  }
   __device__ __forceinline__ bool partial(int g) const {
     return g >= 0 && g < groups && (g < lo || g >= hi);
   }
@@ -266,47 +276,64 @@ struct RowSum {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[u][e] = clean2(w[u][e]);
-        mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w[u][e]));
-      }
+      for (int e = 0; e < 4; ++e) mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w[u][e]));
     }
     const float top = fmaxf(m, fmaxf(__low2float(mx), __high2float(mx)));
-    if (top == -INFINITY) return;
-    if (top == INFINITY) {  // infinite logits share everything
-      if (m < INFINITY) sum = 0.f;
+    if (top == -INFINITY) return;  // nothing but -inf and NaN
+    const float base = top * c;
+    if (!(fabsf(base) < 0x1p24f)) {
+      // infinite, or so steep that the next bf16 is 2^-65536 below: ties of the
+      // largest share everything
+      if (m < top) sum = 0.f;
+      m = top;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          sum += static_cast<float>((w[u][e] & 0xffffu) == 0x7f80u) +
-                 static_cast<float>((w[u][e] >> 16) == 0x7f80u);
+          sum += static_cast<float>(__uint_as_float(w[u][e] << 16) == top) +
+                 static_cast<float>(__uint_as_float(w[u][e] & 0xffff0000u) == top);
       }
-      m = top;
       return;
     }
     sum *= scale_to(m, top, c);
     m = top;
-    const uint64_t ntop2 = pack_f32x2(-top, -top), c2 = pack_f32x2(c, c);
-    const uint64_t zero2 = pack_f32x2(0.f, 0.f);
-    uint64_t acc[2] = {zero2, zero2};
+    // l * c - base in one fma each: base is rounded, by r exactly, alike in all
+    const uint64_t c2 = pack_f32x2(c, c), nbase2 = pack_f32x2(-base, -base);
+    const float r = fmaf(top, c, -base);
+    float a = exps(w, c2, nbase2);
+    if (a != a) {  // NaN logits have no weight
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[u][e] = clean2(w[u][e]);
+      }
+      a = exps(w, c2, nbase2);
+    }
+    sum += a * fast_exp2(-r);
+  }
+
+ private:
+  template <int N>
+  __device__ __forceinline__ static float exps(const uint32_t (&w)[N][4], uint64_t c2,
+                                               uint64_t nbase2) {
+    uint64_t acc[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
     for (int u = 0; u < N; ++u) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint64_t l2 = (static_cast<uint64_t>(w[u][e] & 0xffff0000u) << 32) | (w[u][e] << 16);
-        acc[e & 1] = add_f32x2(acc[e & 1],
-                               exp2_mufu_f32x2(fma_f32x2(add_f32x2(l2, ntop2), c2, zero2)));
+        const uint64_t l2 = pack_f32x2(__uint_as_float(w[u][e] << 16),
+                                       __uint_as_float(w[u][e] & 0xffff0000u));
+        acc[e & 1] = add_f32x2(acc[e & 1], exp2_mufu_f32x2(fma_f32x2(l2, c2, nbase2)));
       }
     }
     const float2 a = unpack_f32x2(add_f32x2(acc[0], acc[1]));
-    sum += a.x + a.y;
+    return a.x + a.y;
   }
 };
 
 // This thread's part of a slice of one row (kRowBatch vectors in flight), or of
 // the target's and the draft's row together (that many of each).
-constexpr int kRowBatch = 5, kRowBatch2 = 3;
+constexpr int kRowBatch = 5, kRowBatch2 = 5;
 
 // The partial groups of a slice, one on each of two threads.
 __device__ __forceinline__ int edge_group(const Slice& s) {
@@ -421,7 +448,7 @@ __device__ __forceinline__ const unsigned short* row_of(const __nv_bfloat16* bas
 }
 
 template <bool kDraft>
-__global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 3) verify_walk_kernel(const VerifyParams p) {
   __shared__ VerifyShared sh;
   __shared__ double table[kExpTable];
   __shared__ int32_t parents[kMaxNodes];
@@ -467,6 +494,20 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const Ve
     const unsigned short* qrow =
         with_q ? row_of(p.draft, b, p.d_stride_seq, node, p.d_stride_row) : prow;
     const Slice ps(prow + x0, len), qs(qrow + x0, with_q ? len : 0);
+    if (tid == 0) {
+      if (count == 0) {  // later rows were sent for at the node before
+        ps.prefetch();
+        qs.prefetch();
+      }
+      // the rows of the likeliest next node, the first child
+      int c = node + 1;
+      while (c < n && parents[c] != node) ++c;
+      if (c < n && p.ahead) {
+        Slice(row_of(p.logits, b, p.l_stride_seq, c, p.l_stride_row) + x0, len).prefetch();
+        if (kDraft && !greedy && c + 1 < n)
+          Slice(row_of(p.draft, b, p.d_stride_seq, c, p.d_stride_row) + x0, len).prefetch();
+      }
+    }
 
     // ---- a candidate child a lane: its token and what the rows say of it
     struct Child {
@@ -538,19 +579,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const Ve
     int next = -1;
 #pragma unroll 1
     for (int exact = 0; exact < 2; ++exact) {
-      const RowScale scale(any ? top : 0u, c64), qscale(any_q ? qtop : 0u, c64);
       if (exact) {
+        const RowScale scale(any ? top : 0u, c64), qscale(any_q ? qtop : 0u, c64);
         double a = 0.0, d = 0.0;
-#pragma unroll 1
+#pragma unroll 4
         for (int i = tid; i < len; i += kVerifyThreads) {
-          const uint32_t pb = __ldg(ps.src + i);
-          if ((pb & 0x7fffu) <= 0x7f80u && pb != 0xff80u)
-            a += exp2_64(scale.log2_weight(__uint_as_float(scale.raise(pb) << 16)), table);
-          if (any_q) {
-            const uint32_t qb = __ldg(qs.src + i);
-            if ((qb & 0x7fffu) <= 0x7f80u && qb != 0xff80u)
-              d += exp2_64(qscale.log2_weight(__uint_as_float(qscale.raise(qb) << 16)), table);
-          }
+          const uint32_t pb = __ldg(ps.src + i), qb = any_q ? __ldg(qs.src + i) : 0u;
+          a += exp2_64(scale.log2_weight(__uint_as_float(scale.raise(pb) << 16)), table);
+          if (any_q) d += exp2_64(qscale.log2_weight(__uint_as_float(qscale.raise(qb) << 16)), table);
         }
         VerifySlot v;
         v.d = make_double2(warp_sum(a), warp_sum(d));
@@ -563,14 +599,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const Ve
         psum = warp_sum(a);
         qsum = warp_sum(d);
       }
-      const double pinv = 1.0 / psum, qinv = 1.0 / qsum;
-      // a logit's probability; none for NaN and -inf
-      auto prob = [&](const RowScale& sc, uint32_t bits, bool live, double inv) {
-        const double w =
-            exp2_64(sc.log2_weight(__uint_as_float(sc.raise(bits) << 16)), table) * inv;
-        return live && (bits & 0x7fffu) <= 0x7f80u && bits != 0xff80u && w > kNothing ? w : 0.0;
+      // a logit's weight beside psum; none for NaN and -inf. In fp32 at least
+      // 2^-100, so that a live logit is told from none.
+      auto weight = [&](uint32_t bits, uint32_t top_bits, float top_l, bool live) {
+        const float l = __uint_as_float(bits << 16);
+        double w = fmax(static_cast<double>(scale_to(l, top_l, c32)), 0x1p-100);
+        if (exact) {
+          const RowScale sc(live ? top_bits : 0u, c64);
+          w = exp2_64(sc.log2_weight(__uint_as_float(sc.raise(bits) << 16)), table);
+        }
+        return live && l > -INFINITY && w > kNothing ? w : 0.0;
       };
-      double left = 1.0;
+      double left = psum;  // of p's weights
       int nrej = 0;  // rejected tokens: lane i holds the i-th and the 32+i-th
       int64_t rej0 = -1, rej1 = -1;
       bool open = false;
@@ -579,8 +619,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const Ve
         const Child k = c0 == node + 1 ? first : child(c0 + lane);
         double here = 0.0, against = 0.0;
         if (!greedy) {  // uniform
-          here = prob(scale, k.pbits, k.in && any, pinv);
-          if (kDraft) against = prob(qscale, k.qbits, k.in && any_q, qinv);
+          here = weight(k.pbits, top, pmax, k.in && any);
+          if (kDraft) against = weight(k.qbits, qtop, qmax, k.in && any_q);
         }
         unsigned todo = __ballot_sync(0xffffffffu, k.mine);
         while (todo && next < 0 && !open) {
@@ -597,9 +637,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_walk_kernel(const Ve
           } else {
             if (!kDraft && __any_sync(0xffffffffu, inside && (rej0 == x || rej1 == x)))
               hc = 0.0;  // a token tried before has no probability left
-            const double bar = uu * (kDraft ? qc : left);
-            ok = bar < hc;
-            open = !exact && hc > 0.0 && fabs(bar - hc) <= 0x1p-14 * (hc + (kDraft ? bar : 1.0));
+            // u q < p over the common denominator; without q: u R < p times psum
+            const double side = kDraft && any_q ? hc * qsum : hc;
+            const double bar = uu * (kDraft ? qc * psum : left);
+            ok = bar < side;
+            open = !exact && hc > 0.0 &&
+                   (fabs(bar - side) <= 0x1p-14 * (side + (kDraft ? bar : psum)) ||
+                    fmax(bar, side) < 0x1p-60);
           }
           if (ok) {
             next = c0 + src;
@@ -881,23 +925,26 @@ static cudaError_t launch_cluster(void (*kernel)(VerifyParams), VerifyParams p, 
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
   cfg.blockDim = dim3(kVerifyThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[3];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
+  attr[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
+  attr[2].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[2].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 2 : 1;
+  cfg.numAttrs = dependent ? 3 : 2;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-#ifndef VWALK
-#define VWALK 4
-#endif
-#ifndef VDRAW
-#define VDRAW 2
-#endif
+// CTAs an SM that size the clusters (fit below). The walk's rows are a chain, so
+// more CTAs a sequence shorten it until they queue for the SMs: 64 sequences of 7
+// drafts take 142, 120 and 138 us with 4, 8 and 16 CTAs each. The draw is bound by
+// fp64: what the SMs hold at once (64 sequences: 4 CTAs each 120 us for both
+// kernels, 8 each 127).
+constexpr int kWalkPerSm = 6, kDrawPerSm = 2;
+
 template <bool kDraft>
 static int launch_verify(const VerifyParams& p, int batch, cudaStream_t stream) {
   static std::mutex mu;
@@ -916,17 +963,20 @@ static int launch_verify(const VerifyParams& p, int batch, cudaStream_t stream) 
       if (dev < 64) done[dev] = true;
     }
   }
-  // CTAs a sequence: as many as the SMs hold for all sequences at once
+  // CTAs a sequence, from the batch alone
   const int64_t sms = device_sm_count();
   auto fit = [&](int per_sm) {
     int ranks = kMaxCluster;
     while (ranks > 2 && static_cast<int64_t>(batch) * ranks > per_sm * sms) ranks /= 2;
     return ranks;
   };
-  cudaError_t e = launch_cluster(verify_walk_kernel<kDraft>, p, batch, fit(VWALK), false, stream);
+  const int ranks = fit(kWalkPerSm);
+  VerifyParams w = p;
+  w.ahead = static_cast<int64_t>(batch) * ranks <= kWalkPerSm * sms;
+  cudaError_t e = launch_cluster(verify_walk_kernel<kDraft>, w, batch, ranks, false, stream);
   if (e != cudaSuccess) return cuda_fail(e, "verify_walk_kernel launch");
   if (p.temperatures == nullptr) return NVATTN_OK;  // all greedy: nothing to draw
-  e = launch_cluster(verify_draw_kernel<kDraft>, p, batch, fit(VDRAW), true, stream);
+  e = launch_cluster(verify_draw_kernel<kDraft>, p, batch, fit(kDrawPerSm), true, stream);
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "verify_draw_kernel launch");
 }
 
