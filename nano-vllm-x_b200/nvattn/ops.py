@@ -131,17 +131,46 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream(device: torch.device) -> int:
-    if _raw_stream is not None and device.index is not None:
-        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
+
+# The newer operators take the device as its index: these calls run per launch,
+# and building torch.device and Stream objects costs microseconds of host time.
 
 _HERE = contextlib.nullcontext()
 
 
-def _device(device: torch.device):
-    """Makes `device` current for a launch (nothing to do when it already is)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _one_device(*tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device that all the tensors are on (None is skipped)."""
+    index = -2
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if i < 0 or index >= 0:
+                    _require_cuda(*tensors)  # raises
+                index = i
+    return index
+
+
+def _on_device(index: int):
+    """Makes a device current for a launch (nothing to do when it already is)."""
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+_status_ptrs: dict[int, int] = {}
+
+
+def _launch_args(index: int) -> tuple[int | None, int]:
+    """Status word and current stream of a device."""
+    status = _status_ptrs.get(index)
+    if status is None:
+        t = status_tensor(index)
+        if t is not None:
+            status = _status_ptrs[index] = t.data_ptr()
+    if _raw_stream is not None:
+        return status, _raw_stream(index)
+    return status, torch.cuda.current_stream(index).cuda_stream
 
 
 def _check_bf16(*tensors: torch.Tensor) -> None:
@@ -161,9 +190,10 @@ def _check_table(block_table: torch.Tensor, rows: int) -> None:
     """An int32 (rows, W) block table; rows may be strided (a slice of a wider table)."""
     if block_table.dtype != torch.int32:
         raise TypeError(f"block_table must be int32, got {block_table.dtype}")
-    if block_table.dim() != 2 or block_table.shape[0] != rows:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != rows:
         raise ValueError("block_table needs one row per sequence")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    if block_table.stride(1) != 1 and shape[1] > 1:
         raise ValueError("block_table rows must be contiguous")
 
 
@@ -191,13 +221,14 @@ def _check_decode(q: torch.Tensor, out: torch.Tensor | None, cache_seqlens: torc
     return batch, num_heads, head_dim, out
 
 
-def _workspace(need: int, workspace: torch.Tensor | None, device: torch.device):
-    """(pointer, bytes) of the caller's workspace, or of a new one of `need` bytes."""
+def _workspace(need: int, workspace: torch.Tensor | None, like: torch.Tensor):
+    """(pointer, bytes, tensor) of the caller's workspace, or of a new one of `need` bytes; the
+    tensor is held until the launch, so that the allocator gives it to no other thread."""
     if not need:
-        return None, 0
+        return None, 0, None
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        workspace = like.new_empty(need, dtype=torch.uint8)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 # --------------------------------------------------------------------- scatter
@@ -386,23 +417,23 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, cache_seqlens=None, block_table
 # ------------------------------------------------------------------- fp8 cache
 
 def _check_fp8_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
-                      v_scale: torch.Tensor) -> tuple[int, int, int]:
-    """Shapes of an fp8 cache and its exponents; returns (num_blocks, block_size, kv_heads)."""
+                      v_scale: torch.Tensor) -> tuple[int, int, int, int]:
+    """Checks an fp8 cache and its exponents; returns the caches' shape."""
     if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise TypeError("fp8 caches must be float8_e4m3fn, got "
                         f"{k_cache.dtype} and {v_cache.dtype}")
     if k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
         raise TypeError("k_scale and v_scale must be uint8 exponent bytes")
-    shape = k_cache.shape
+    shape, scales = k_cache.shape, k_scale.shape
     if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("caches must be (num_blocks, block_size, kv_heads, d)")
-    num_blocks, block_size, num_kv_heads, _ = shape
-    if k_scale.shape != (num_blocks, num_kv_heads, block_size) or v_scale.shape != k_scale.shape:
+    num_blocks, block_size, num_kv_heads, head_dim = shape
+    if scales != (num_blocks, num_kv_heads, block_size) or scales != v_scale.shape:
         raise ValueError("k_scale and v_scale must be (num_blocks, kv_heads, block_size)")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
         raise ValueError("fp8 caches and their scales must be contiguous")
-    return num_blocks, block_size, num_kv_heads
+    return num_blocks, block_size, num_kv_heads, head_dim
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -418,23 +449,23 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     most 448; a row with a value that is not finite reads back as NaN. Slot -1
     is skipped; the other slots of a call must be distinct.
     """
-    N, num_heads, head_dim = key.shape
-    dev = _require_cuda(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    dev = _one_device(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     _check_bf16(key, value)
     _check_i32("slot_mapping", slot_mapping)
-    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
-    if value.shape != key.shape or (num_heads, head_dim) != (num_kv_heads, k_cache.shape[3]):
+    num_blocks, block_size, num_kv_heads, d = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    shape = key.shape
+    if len(shape) != 3 or shape != value.shape or shape[1] != num_kv_heads or shape[2] != d:
         raise ValueError("key/value must be (N, kv_heads, d) like the caches' rows")
-    for n, t in (("key", key), ("value", value)):
-        if t.stride(2) != 1 or (num_heads > 1 and t.stride(1) != head_dim):
-            raise ValueError(f"{n} must have unit element stride and head stride head_dim")
-    if slot_mapping.numel() != N:
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1 or vs[2] != 1 or (num_kv_heads > 1 and (ks[1] != d or vs[1] != d)):
+        raise ValueError("key/value must have unit element stride and head stride head_dim")
+    if slot_mapping.numel() != shape[0]:
         raise ValueError("slot_mapping must have one entry per token")
-    with _device(dev):
-        _lib.call("nvattn_store_kvcache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(),
-                  value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                  v_scale.data_ptr(), slot_mapping.data_ptr(), N, num_kv_heads, head_dim,
-                  num_blocks, block_size, _status_ptr(dev), _stream(dev))
+    with _on_device(dev):
+        _lib.call("nvattn_store_kvcache_fp8", key.data_ptr(), ks[0], value.data_ptr(), vs[0],
+                  k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  slot_mapping.data_ptr(), shape[0], num_kv_heads, d, num_blocks, block_size,
+                  *_launch_args(dev))
 
 
 def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -448,30 +479,30 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     int32) lands in row cu_seqlens_k[b] + j; rows behind the last sequence are
     left as they were in a given k_out and v_out, and zeros in new ones.
     """
-    dev = _require_cuda(k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_table, k_out,
-                        v_out)
+    dev = _one_device(k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_table, k_out, v_out)
     _check_i32("cu_seqlens_k", cu_seqlens_k)
-    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    num_blocks, block_size, num_kv_heads, d = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
     num_seqs = cu_seqlens_k.numel() - 1
     _check_table(block_table, num_seqs)
-    head_dim = k_cache.shape[3]
-    shape = (int(total_k), num_kv_heads, head_dim)
+    total_k = int(total_k)
+    shape = (total_k, num_kv_heads, d)
     new = k_out is None
     if new != (v_out is None):
         raise ValueError("give both k_out and v_out, or neither")
     if new:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    _check_bf16(k_out, v_out)
-    for n, t in (("k_out", k_out), ("v_out", v_out)):
-        if t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{n} must be contiguous {shape}")
-    with _device(dev):
+        k_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
+        v_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
+    else:
+        _check_bf16(k_out, v_out)
+        for n, t in (("k_out", k_out), ("v_out", v_out)):
+            if t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{n} must be contiguous {shape}")
+    with _on_device(dev):
         _lib.call("nvattn_load_kvcache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
                   k_scale.data_ptr(), v_scale.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs,
                   block_table.data_ptr(), block_table.stride(0), block_table.shape[1], num_blocks,
-                  block_size, num_kv_heads, head_dim, int(total_k), 1 if new else 0, k_out.data_ptr(),
-                  v_out.data_ptr(), _status_ptr(dev), _stream(dev))
+                  block_size, num_kv_heads, d, total_k, 1 if new else 0, k_out.data_ptr(),
+                  v_out.data_ptr(), *_launch_args(dev))
     return k_out, v_out
 
 
@@ -490,23 +521,23 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     ``workspace``: uint8, ``decode_fp8_workspace_bytes`` of the same sizes.
     """
-    dev = _require_cuda(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, out,
-                        workspace)
-    num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
+    dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, out,
+                      workspace)
+    num_blocks, block_size, num_kv_heads, d = _check_fp8_caches(k_cache, v_cache, k_scale, v_scale)
     batch, num_heads, head_dim, out = _check_decode(q, out, cache_seqlens, block_table,
-                                                    num_kv_heads, k_cache.shape[3])
+                                                    num_kv_heads, d)
     max_blocks = block_table.shape[1]
-    with _device(dev):
-        ws_ptr, ws_bytes = _workspace(decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads,
+    with _on_device(dev):
+        ws_ptr, ws_bytes, _ws = _workspace(decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads,
                                                                  max_blocks, block_size),
-                                      workspace, dev)
+                                      workspace, q)
         _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),
                   block_table.data_ptr(), block_table.stride(0), max_blocks, num_blocks,
                   block_size, batch, num_heads, num_kv_heads, head_dim,
                   head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
-                  ws_bytes, _status_ptr(dev), _stream(dev))
+                  ws_bytes, *_launch_args(dev))
     return out
 
 
@@ -533,28 +564,28 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
     ``workspace``: uint8, ``shared_prefix_workspace_bytes`` of the same sizes.
     """
-    dev = _require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out,
-                        workspace)
+    dev = _one_device(q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out,
+                      workspace)
     fp8 = k_scale is not None
     if fp8 != (v_scale is not None):
         raise ValueError("give both k_scale and v_scale, or neither")
     if fp8:
-        num_blocks, block_size, num_kv_heads = _check_fp8_caches(k_cache, v_cache, k_scale,
-                                                                 v_scale)
+        num_blocks, block_size, num_kv_heads, d = _check_fp8_caches(k_cache, v_cache, k_scale,
+                                                                    v_scale)
     else:
         _check_bf16(k_cache, v_cache)
         if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
             raise ValueError("caches must be (num_blocks, block_size, kv_heads, d)")
         if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
             raise ValueError("caches must be contiguous")
-        num_blocks, block_size, num_kv_heads = k_cache.shape[:3]
+        num_blocks, block_size, num_kv_heads, d = k_cache.shape
     batch, num_heads, head_dim, out = _check_decode(q, out, cache_seqlens, block_table,
-                                                    num_kv_heads, k_cache.shape[3])
+                                                    num_kv_heads, d)
     shared_len, max_blocks = int(shared_len), block_table.shape[1]
-    with _device(dev):
-        ws_ptr, ws_bytes = _workspace(
+    with _on_device(dev):
+        ws_ptr, ws_bytes, _ws = _workspace(
             shared_prefix_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size,
-                                          shared_len, fp8), workspace, dev)
+                                          shared_len, fp8), workspace, q)
         _lib.call("nvattn_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if fp8 else None,
                   v_scale.data_ptr() if fp8 else None, out.data_ptr(), out.stride(0),
@@ -562,7 +593,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                   block_table.stride(0), max_blocks, num_blocks, block_size, shared_len, batch,
                   num_heads, num_kv_heads, head_dim,
                   head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
-                  ws_bytes, _status_ptr(dev), _stream(dev))
+                  ws_bytes, *_launch_args(dev))
     return out
 
 
@@ -826,8 +857,8 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: tor
     ``tree.compaction_moves``; accepted (B,) int32). The tokens follow the
     target's law; every decision is that of 64-bit arithmetic.
     """
-    dev = _require_cuda(logits, draft_tokens, u_accept, u_pick, temperatures, draft_logits,
-                        parents, num_nodes)
+    dev = _one_device(logits, draft_tokens, u_accept, u_pick, temperatures, draft_logits, parents,
+                      num_nodes)
     _check_bf16(logits, draft_logits)
     if logits.dim() != 3 or logits.stride(2) != 1:
         raise ValueError("logits must be (B, n, V) with unit column stride")
@@ -851,10 +882,10 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: tor
         if draft_logits.shape != (B, n - 1, V) or (n > 1 and draft_logits.stride(2) != 1):
             raise ValueError("draft_logits must be (B, n - 1, V) with unit column stride")
         d_strides = draft_logits.stride()[:2]
-    tokens = torch.empty((B, n), dtype=torch.int64, device=dev)
-    path = torch.empty((B, n), dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    with _device(dev):
+    tokens = logits.new_empty((B, n), dtype=torch.int64)
+    path = logits.new_empty((B, n), dtype=torch.int32)
+    accepted = logits.new_empty(B, dtype=torch.int32)
+    with _on_device(dev):
         _lib.call("nvattn_verify_draft", logits.data_ptr(), logits.stride(0), logits.stride(1),
                   draft_logits.data_ptr() if draft_logits is not None and n > 1 else None,
                   *d_strides, draft_tokens.data_ptr(),
@@ -862,5 +893,5 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: tor
                   parents.stride(0) if parents is not None else 0, u_accept.data_ptr(),
                   u_pick.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
                   num_nodes.data_ptr() if num_nodes is not None else None, B, n, V,
-                  tokens.data_ptr(), path.data_ptr(), accepted.data_ptr(), _stream(dev))
+                  tokens.data_ptr(), path.data_ptr(), accepted.data_ptr(), _launch_args(dev)[1])
     return tokens, path, accepted
