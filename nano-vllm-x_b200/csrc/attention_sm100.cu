@@ -716,7 +716,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t orr[32];
       sm100::tmem_ld32(t_lane + col_o(wg) + c * 32, orr);
       sm100::tmem_wait_ld();
-      if (valid && done && (MODE == kShared || p.nsplit > 1)) {
+      if (MODE == kShared) {
+        // 32 rows x 32 columns through the K/V ring (every copy and MMA on it is
+        // done): a warp then writes 128 bytes of 4 rows at a time, not 16 of 32
+        float* buf = reinterpret_cast<float*>(smem + kQBytes) + (warp - 2) * 32 * 36;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<float4*>(buf + lane * 36 + 4 * e) =
+              make_float4(__uint_as_float(orr[4 * e]), __uint_as_float(orr[4 * e + 1]),
+                          __uint_as_float(orr[4 * e + 2]), __uint_as_float(orr[4 * e + 3]));
+        const int64_t slot =
+            valid && done ? (static_cast<int64_t>(tok) * p.num_heads + g * group + hh) * p.nsplit + split
+                          : -1;
+        if (c == 0 && slot >= 0) p.ws_ml[slot] = make_float2(m_used, l);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int rr = e * 4 + (lane >> 3), cc = (lane & 7) * 4;
+          const int64_t to = __shfl_sync(0xffffffffu, slot, rr);
+          if (to >= 0)
+            *reinterpret_cast<float4*>(p.ws_o + to * kHeadDim + c * 32 + cc) =
+                *reinterpret_cast<const float4*>(buf + rr * 36 + cc);
+        }
+        __syncwarp();
+      } else if (valid && done && p.nsplit > 1) {
         const int64_t slot =
             (static_cast<int64_t>(q_begin + tok) * p.num_heads + g * group + hh) * p.nsplit + split;
         float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * kHeadDim + c * 32);

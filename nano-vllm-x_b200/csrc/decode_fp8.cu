@@ -40,16 +40,11 @@ namespace nvattn {
 namespace cg = cooperative_groups;
 
 constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
-// Consumer warps of a CTA and CTAs of an SM for NB blocks of 8 query heads
-// (registers a thread grow with NB).
-#ifndef DEC8W
-#define DEC8W 4
-#endif
-#ifndef DEC8C
-#define DEC8C 3
-#endif
-constexpr int dec8_warps(int NB) { return NB == 1 ? DEC8W : 4; }
-constexpr int dec8_ctas(int NB) { return NB == 1 ? DEC8C : 2; }
+// Warps of a CTA and CTAs of an SM for NB blocks of 8 query heads (registers a
+// thread grow with NB). 256 sequences of 100 to 2048 keys: 4 warps x 3 CTAs 88 us;
+// 6 x 2 91, 3 x 4 92, 2 x 6 94.
+constexpr int dec8_warps(int) { return 4; }
+constexpr int dec8_ctas(int NB) { return NB == 1 ? 3 : 2; }
 
 // Shared memory of one warp: its K and V tile, their exponent bytes.
 constexpr int kWarpBytes8 = 2 * kTile8;
