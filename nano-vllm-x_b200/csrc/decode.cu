@@ -33,13 +33,9 @@ constexpr int kDecStages = 3;                  // ring depth
 constexpr int kHalfBytes = kTile * 128;        // one 64-token x 64-dim half tile (8 KB)
 constexpr int kStageBytes = 4 * kHalfBytes;    // K lo/hi + V lo/hi (32 KB)
 // Split policy (see choose_split); overridable at build time for tuning sweeps.
-#ifndef NVATTN_DEC_MIN_SPLIT_TILES
-#define NVATTN_DEC_MIN_SPLIT_TILES 4
-#endif
 #ifndef NVATTN_DEC_SPLIT_CTAS_PER_SM
 #define NVATTN_DEC_SPLIT_CTAS_PER_SM 8
 #endif
-constexpr int kMinSplitTiles = NVATTN_DEC_MIN_SPLIT_TILES;
 constexpr int kSplitCtasPerSm = NVATTN_DEC_SPLIT_CTAS_PER_SM;
 
 // kSuffix: the row's keys behind a shared prefix, as fp32 partials
@@ -366,12 +362,12 @@ int device_sm_count() {
 // writes the output itself and no combine runs).
 // Depends only on host-side sizes, so a captured graph keeps its grid.
 void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size, int* nsplit,
-                  int* split_tiles) {
+                  int* split_tiles, int min_tiles) {
   const int sms = device_sm_count();
   const int64_t max_tiles = (static_cast<int64_t>(max_blocks) * block_size + kTile - 1) / kTile;
   const int64_t pairs = static_cast<int64_t>(batch) * num_kv_heads;
   int st = 64;
-  while (st > kMinSplitTiles) {
+  while (st > min_tiles) {
     const int64_t ns = (max_tiles + st - 1) / st;
     if (pairs * ns >= static_cast<int64_t>(kSplitCtasPerSm) * sms) break;
     st >>= 1;

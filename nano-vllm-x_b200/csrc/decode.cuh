@@ -7,6 +7,10 @@
 namespace nvattn {
 
 constexpr int kTile = 64;                      // tokens per pipeline stage
+// Smallest split of decode.cu; overridable at build time for tuning sweeps.
+#ifndef NVATTN_DEC_MIN_SPLIT_TILES
+#define NVATTN_DEC_MIN_SPLIT_TILES 4
+#endif
 constexpr int kDecConsumerWarps = 4;
 constexpr int kDecThreads = (kDecConsumerWarps + 1) * 32;
 constexpr int kMaxGroup = 16;                  // query heads per KV head handled per CTA
@@ -54,9 +58,11 @@ __device__ __forceinline__ void join_prefix_grid() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Split size for a batch over tables of max_blocks (see decode.cu).
+// Split size for a batch over tables of max_blocks, of at least min_tiles (see
+// decode.cu).
+constexpr int kMinSplitTiles = NVATTN_DEC_MIN_SPLIT_TILES;
 void choose_split(int batch, int num_kv_heads, int max_blocks, int block_size, int* nsplit,
-                  int* split_tiles);
+                  int* split_tiles, int min_tiles = kMinSplitTiles);
 // Splits of the fp8 kernel for rows of up to max_keys, and the cluster that
 // merges them (decode_fp8.cu).
 void choose_split_fp8(int batch, int num_kv_heads, int64_t max_keys, int* nsplit, int* split_tiles,
