@@ -21,7 +21,8 @@ scatters K/V (qwen3.py:82-86 and attention.py:62-63) before the attention.
 The cache may also be bound as ``float8_e4m3fn`` pages with their exponent
 bytes in ``k_scale``/``v_scale`` (``ops.store_kvcache_fp8``): new rows are then
 quantised as they are scattered, decode attends the fp8 pages, and a
-prefix-cache prefill reads its sequences back as dense bf16 rows first.
+prefix-cache prefill reads its sequences back as dense bf16 rows first, a group
+of sequences at a time so that these rows stay within about ``READ_BACK_KEYS``.
 
 All steps run libnvattn kernels; there is no other code path.
 """
@@ -32,6 +33,11 @@ from torch import nn
 
 from . import context as _ctx
 from . import ops
+
+
+# Keys per group of sequences that a prefill over an fp8 cache reads back (1 GB
+# for 8 KV heads; one sequence may be longer)
+READ_BACK_KEYS = 1 << 18
 
 
 class Attention(nn.Module):
@@ -56,7 +62,11 @@ class Attention(nn.Module):
         return self._attend(context, q, k, v)
 
     def _fp8(self) -> bool:
-        return self.k_cache.dtype == torch.float8_e4m3fn
+        if self.k_cache.dtype != torch.float8_e4m3fn:
+            return False
+        if self.k_scale is None or self.v_scale is None:
+            raise ValueError("an fp8 cache needs its exponent bytes in k_scale and v_scale")
+        return True
 
     def _store(self, k, v, slot_mapping):
         if self._fp8():
@@ -93,22 +103,14 @@ class Attention(nn.Module):
     def _attend(self, context, q: torch.Tensor, k, v):
         k_cache, v_cache = self.k_cache, self.v_cache
         if context.is_prefill:
-            block_table = context.block_tables
-            if block_table is not None:  # prefix cache
-                k, v = k_cache, v_cache
+            if context.block_tables is not None:  # prefix cache
                 if self._fp8():
-                    # no sequence has more keys than its table holds or than
-                    # max_seqlen_k: an upper bound of cu_seqlens_k[-1] without
-                    # reading it back from the device
-                    total_k = block_table.shape[0] * min(context.max_seqlen_k,
-                                                         block_table.shape[1] * k_cache.shape[1])
-                    k, v = ops.load_kvcache_fp8(k_cache, v_cache, self.k_scale, self.v_scale,
-                                                context.cu_seqlens_k, block_table, total_k)
-                    block_table = None
+                    return self._prefill_fp8(context, q)
+                k, v = k_cache, v_cache
             o = ops.varlen_prefill(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
                                    context.max_seqlen_q, context.max_seqlen_k,
                                    softmax_scale=self.scale, causal=True,
-                                   block_table=block_table)
+                                   block_table=context.block_tables)
         elif self._fp8():
             o = ops.paged_decode_fp8(q, k_cache, v_cache, self.k_scale, self.v_scale,
                                      context.context_lens, context.block_tables,
@@ -116,4 +118,25 @@ class Attention(nn.Module):
         else:  # decode
             o = ops.paged_decode(q, k_cache, v_cache, context.context_lens,
                                  context.block_tables, softmax_scale=self.scale).unsqueeze(1)
+        return o
+
+    def _prefill_fp8(self, context, q: torch.Tensor) -> torch.Tensor:
+        """Prefix-cache prefill over an fp8 cache: the sequences' rows read back, then dense.
+
+        The rows' number is on the device only, so each group of sequences gets
+        room for max_seqlen_k (or a full table) apiece: ragged batches would
+        claim many times their keys if all were read back at once.
+        """
+        table, cu_q, cu_k = context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k
+        longest = max(1, min(context.max_seqlen_k, table.shape[1] * self.k_cache.shape[1]))
+        step = max(1, READ_BACK_KEYS // longest)
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        for b in range(0, table.shape[0], step):
+            rows = table[b:b + step]
+            ck = cu_k[b:b + step + 1]
+            ck = ck - ck[0]
+            k, v = ops.load_kvcache_fp8(self.k_cache, self.v_cache, self.k_scale, self.v_scale,
+                                        ck, rows, rows.shape[0] * longest)
+            ops.varlen_prefill(q, k, v, cu_q[b:b + step + 1], ck, context.max_seqlen_q,
+                               context.max_seqlen_k, softmax_scale=self.scale, causal=True, out=o)
         return o

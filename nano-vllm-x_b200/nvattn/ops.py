@@ -490,8 +490,9 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     if new != (v_out is None):
         raise ValueError("give both k_out and v_out, or neither")
     if new:
-        k_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
-        v_out = k_cache.new_empty(shape, dtype=torch.bfloat16)
+        make = k_cache.new_empty if num_seqs else k_cache.new_zeros  # no sequence: all rows zero
+        k_out = make(shape, dtype=torch.bfloat16)
+        v_out = make(shape, dtype=torch.bfloat16)
     else:
         _check_bf16(k_out, v_out)
         for n, t in (("k_out", k_out), ("v_out", v_out)):
@@ -528,9 +529,9 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                                                     num_kv_heads, d)
     max_blocks = block_table.shape[1]
     with _on_device(dev):
-        ws_ptr, ws_bytes, _ws = _workspace(decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads,
-                                                                 max_blocks, block_size),
-                                      workspace, q)
+        ws_ptr, ws_bytes, _ws = _workspace(
+            decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size),
+            workspace, q)
         _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),

@@ -413,3 +413,74 @@ def test_attention_module_with_an_fp8_cache():
         check(o[:, 0], ref, mag, "module step")
     ctxmod.reset_context()
     assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("keys", [1, 700, 1 << 18])
+def test_module_prefill_reads_back_in_groups(monkeypatch, keys):
+    """A ragged prefix-cache prefill over an fp8 cache, read back one sequence at a time, two at a
+    time and all together (one sequence has no new tokens)."""
+    from nvattn import attention as attention_module
+    monkeypatch.setattr(attention_module, "READ_BACK_KEYS", keys)
+    H, KVH, bs = 4, 2, 64
+    g = torch.Generator().manual_seed(77)
+    tot, add = [300, 1, 130, 64, 257], [7, 1, 0, 64, 33]
+    attn = nvattn.Attention(H, 128, SCALE, KVH)
+    caches, bt = [], torch.arange(30, dtype=torch.int32).flip(0).view(5, 6)[:, :5].contiguous()
+    for name in "kv":
+        q, e = filled_cache(30, bs, KVH, g)
+        caches.append(R.expand_cache_fp8(q, e))
+        setattr(attn, f"{name}_cache", q.to(dev))
+        setattr(attn, f"{name}_scale", e.to(dev))
+    n = sum(add)
+    q, k, v = [torch.randn(n, h, 128, generator=g).to(torch.bfloat16) for h in (H, KVH, KVH)]
+    cq, ck = cu(add), cu(tot)
+    skip = torch.full((n,), -1, dtype=torch.int32, device=dev)  # the keys are there already
+    ctxmod.set_context(True, cq.to(dev), ck.to(dev), max(add), max(tot), skip, None, bt.to(dev))
+    ops.read_status()
+    o = attn(q.to(dev), k.to(dev), v.to(dev))
+    ctxmod.reset_context()
+    kv = [torch.cat([R.gather_paged(c, bt[b].numpy(), m) for b, m in enumerate(tot)]).to(torch.bfloat16)
+          for c in caches]
+    ref = R.varlen_attention(q, *kv, cq.numpy(), ck.numpy(), SCALE, True)
+    assert (o.float().cpu() - ref).abs().max() <= 1e-2 + 2.0 ** -8 * ref.abs().max()
+    assert ops.read_status() == 0
+
+
+def test_module_fused_step_equals_the_separate_one():
+    """forward_fused bound to an fp8 cache: its cache bytes and outputs are those of forward on the
+    normalised, rotated q and k."""
+    H, KVH, bs, n = 8, 2, 64, 3
+    g = torch.Generator().manual_seed(78)
+    qkv = torch.randn(n, (H + 2 * KVH) * 128, generator=g).to(torch.bfloat16).to(dev)
+    q, k, v = [t.view(n, -1, 128) for t in qkv.split([H * 128, KVH * 128, KVH * 128], -1)]
+    w = torch.randn(2, 128, generator=g).to(torch.bfloat16).to(dev)
+    angles = torch.rand(100, 1, 64, generator=g)
+    table = torch.cat([angles.cos(), angles.sin()], -1).to(dev)
+    pos = torch.tensor([0, 70, 33], device=dev)
+    bt = torch.tensor([[5, 0], [1, 4], [3, 2]], dtype=torch.int32, device=dev)
+    slots = torch.tensor([5 * bs, 4 * bs + 6, 3 * bs + 33], dtype=torch.int32, device=dev)
+    lens = torch.tensor([1, 71, 34], dtype=torch.int32, device=dev)
+    start = [filled_cache(6, bs, KVH, g) for _ in "kv"]
+    results = []
+    for fused in (True, False):
+        attn = nvattn.Attention(H, 128, SCALE, KVH)
+        (attn.k_cache, attn.k_scale), (attn.v_cache, attn.v_scale) = [
+            (c.to(dev), s.to(dev)) for c, s in start]
+        ctxmod.set_context(False, slot_mapping=slots, context_lens=lens, block_tables=bt)
+        if fused:
+            o = attn.forward_fused(pos, q, k, v, w[0], w[1], table, 1e-6)
+        else:
+            o = attn(*ops.qk_norm_rope_store(pos, q, k, v, w[0], w[1], table, 1e-6), v)
+        results.append([o, u8(attn.k_cache), u8(attn.v_cache), attn.k_scale, attn.v_scale])
+    ctxmod.reset_context()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    changed = (results[0][1] != u8(start[0][0]).to(dev)).flatten(2).any(-1).view(-1).nonzero()
+    assert set(changed.flatten().tolist()) <= set(slots.tolist()) and len(changed)
+
+
+def test_load_of_no_sequences_gives_zeros():
+    kc, ks = empty_cache(2, 64, 3)
+    none = torch.zeros(1, dtype=torch.int32, device=dev)
+    k, v = ops.load_kvcache_fp8(kc, kc, ks, ks, none, none.new_empty(0, 4), 5)
+    assert k.shape == (5, 3, 128) and not k.any() and not v.any()

@@ -130,3 +130,12 @@ def test_operators_refuse_cpu_tensors_and_wrong_types():
     with pytest.raises(TypeError, match="int32"):
         ops._check_table(i32.view(3, 1).long(), 3)
     assert np.array_equal(kc.shape, (2, 64, 2, 128))
+
+
+def test_module_needs_the_exponents_of_an_fp8_cache():
+    import nvattn
+    attn = nvattn.Attention(4, 128, 0.1, 2)
+    attn.k_cache = attn.v_cache = torch.zeros(2, 64, 2, 128, dtype=torch.float8_e4m3fn)
+    x = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="k_scale"):
+        attn(x, x, x)
