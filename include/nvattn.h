@@ -41,10 +41,20 @@
  *   dist.all_reduce(y) of RowParallelLinear      -> nvattn_allreduce
  *     (+ nvattn_ar_buffer_bytes / _alloc / _open / _close / _free)
  *
+ * and entry points with no counterpart in the reference, for serving:
+ *
+ *   nvattn_store_kvcache_fp8     the cache in 8-bit floating point: scatter with
+ *   nvattn_load_kvcache_fp8      quantisation, read-back as dense bf16 rows,
+ *   nvattn_paged_decode_fp8      decode attention
+ *   nvattn_shared_prefix_decode  decode attention with the keys that a batch
+ *                                shares read once (bf16 or fp8 cache)
+ *   nvattn_verify_draft          which drafted tokens stand, and the next token
+ *
  * Conventions (all entry points):
  *   - Pointers are device pointers unless stated otherwise; no torch types.
  *   - Strides are in ELEMENTS (like torch.Tensor.stride()).
- *   - Element type is bf16 (2 bytes); head_dim must be 128.
+ *   - Element type is bf16 (2 bytes), in the fp8 entries' caches e4m3 (1 byte);
+ *     head_dim must be 128.
  *   - KV cache layout is the engine's (nanovllm/engine/model_runner.py:115):
  *     one layer's cache is [num_blocks][block_size][num_kv_heads][head_dim],
  *     contiguous; slot s lives at row s of the [num_blocks*block_size]
@@ -249,11 +259,13 @@ NVATTN_API int nvattn_paged_decode_noalloc(const void* q, int64_t q_stride_tok, 
  * up to 127 rows behind a sequence's keys, masked: they must be finite); keys
  * whose block id or table column is out of range
  * become zeros and set NVATTN_STATUS_BAD_BLOCK. cu_seqlens_k must not decrease.
+ * num_seqs 0: nothing is written.
  *
  * nvattn_paged_decode_fp8 is nvattn_paged_decode over these caches, with the
- * same sizes and limits and a workspace of nvattn_decode_fp8_workspace_bytes (0
- * for short tables: NULL will do); scores and sums are fp32 and the output is
- * rounded to bf16 once. Scales must be 16-byte aligned.
+ * same sizes and limits (and tables of up to 2^30 keys) and a workspace of
+ * nvattn_decode_fp8_workspace_bytes (0 for short tables: NULL will do); scores
+ * and sums are fp32 and the output is rounded to bf16 once. Scales must be
+ * 16-byte aligned.
  */
 NVATTN_API int nvattn_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
                                         int64_t value_stride, void* k_cache, void* v_cache,
@@ -297,7 +309,8 @@ NVATTN_API int nvattn_paged_decode_fp8(
  * shared_len keys (0: a padding row, whose output is zeros) is attended over
  * its own pages alone. shared_len is a multiple of block_size (0: none shared),
  * block_size one of 128. k_scale and v_scale NULL: bf16 caches; otherwise fp8
- * caches as for nvattn_paged_decode_fp8. q rows are 16-byte aligned.
+ * caches as for nvattn_paged_decode_fp8. q rows are 16-byte aligned; tables
+ * cover up to 2^30 keys.
  *
  * `workspace` (device, 256-byte aligned, >= nvattn_shared_prefix_workspace_bytes
  * of the same sizes; fp8 = 0 or 1) holds fp32 partials of both parts and, for an

@@ -89,6 +89,8 @@ int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const v
                              bool after_prefix, cudaStream_t stream);
 // Checks an fp8 cache's scale pointers.
 int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale);
+// Key positions are 32-bit: a table may cover up to 2^30 keys.
+int check_table_keys(const char* who, int32_t max_blocks_per_seq, int32_t block_size);
 // Merges partials of up to two key ranges into p.out: `first` (nfirst of them, all
 // live in a row with keys; p.key_begin keys together) and p's own nsplit ones.
 int launch_merge_partials(const DecodeParams& p, const float* first_o, const float2* first_ml,

@@ -685,6 +685,12 @@ int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale) 
   return NVATTN_OK;
 }
 
+int check_table_keys(const char* who, int32_t max_blocks_per_seq, int32_t block_size) {
+  if (static_cast<int64_t>(max_blocks_per_seq) * block_size > (1 << 30))
+    return fail(NVATTN_ERR_UNSUPPORTED, std::string(who) + ": table of more than 2^30 keys");
+  return NVATTN_OK;
+}
+
 }  // namespace nvattn
 
 using namespace nvattn;
@@ -719,6 +725,8 @@ extern "C" int nvattn_paged_decode_fp8(
                              num_kv_heads, head_dim);
   if (rc) return rc;
   rc = check_fp8_scales("paged_decode_fp8", k_scale, v_scale);
+  if (rc) return rc;
+  rc = check_table_keys("paged_decode_fp8", max_blocks_per_seq, block_size);
   if (rc) return rc;
   if (batch > 65535) return fail(NVATTN_ERR_UNSUPPORTED, "paged_decode_fp8: batch > 65535");
 

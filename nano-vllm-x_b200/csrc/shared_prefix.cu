@@ -96,6 +96,8 @@ extern "C" int nvattn_shared_prefix_decode(
                              cache_seqlens, block_table, block_table_stride, max_blocks_per_seq,
                              num_blocks, block_size, batch, num_heads, num_kv_heads, head_dim);
   if (rc) return rc;
+  rc = check_table_keys(who, max_blocks_per_seq, block_size);
+  if (rc) return rc;
   const bool fp8 = k_scale != nullptr || v_scale != nullptr;
   if (fp8) {
     rc = check_fp8_scales(who, k_scale, v_scale);

@@ -289,3 +289,39 @@ def test_speculative_step_over_an_fp8_cache_with_a_shared_prefix():
             src, dst = tree.compaction_moves(lens[b], nodes, bt[b].tolist(), bs)
             assert len(src) == len(dst)
     assert ops.read_status() == 0
+
+
+def test_pages_whose_offsets_pass_32_bits():
+    """Caches of more than 2^32 bytes: pages at their far end give what the same rows in a small
+    cache give, bit for bit, in every operator over them."""
+    bs, kvh, H, d = 256, 8, 16, 128
+    far = 2 ** 33 // (bs * kvh * d) + 7  # bytes of an fp8 cache; a bf16 one has twice as many
+    lens = torch.tensor([700, 300, 513], dtype=torch.int32, device=dev)
+    small = torch.tensor([[2, 0, 5], [2, 3, -1], [2, 1, 4]], dtype=torch.int32, device=dev)
+    moved = torch.where(small >= 0, far - 1 - small, small)
+    g = torch.Generator().manual_seed(90)
+    n = 6 * bs
+    k, v = [torch.randn(n, kvh, d, generator=g).to(torch.bfloat16).to(dev) for _ in "kv"]
+    q = torch.randn(3, H, d, generator=g).to(torch.bfloat16).to(dev)
+    slots = torch.arange(n, dtype=torch.int32, device=dev)
+    results = []
+    ops.read_status()
+    for blocks, table in ((6, small), (far, moved)):
+        rows = slots if blocks == 6 else (far - 1 - slots // bs) * bs + slots % bs
+        kc, vc = [torch.empty(blocks, bs, kvh, d, dtype=torch.float8_e4m3fn, device=dev) for _ in "kv"]
+        ks, vs = [torch.empty(blocks, kvh, bs, dtype=torch.uint8, device=dev) for _ in "kv"]
+        ops.store_kvcache_fp8(k, v, kc, vc, ks, vs, rows.int())
+        cu_k = torch.tensor([0, 700, 1000, 1513], dtype=torch.int32, device=dev)
+        out = list(ops.load_kvcache_fp8(kc, vc, ks, vs, cu_k, table, 1513))
+        out.append(ops.paged_decode_fp8(q, kc, vc, ks, vs, lens, table))
+        out.append(ops.shared_prefix_decode(q, kc, vc, lens, table, bs, k_scale=ks, v_scale=vs))
+        del kc, vc, ks, vs
+        kc, vc = [torch.empty(blocks, bs, kvh, d, dtype=torch.bfloat16, device=dev) for _ in "kv"]
+        ops.store_kvcache(k, v, kc, vc, rows.int())
+        out.append(ops.shared_prefix_decode(q, kc, vc, lens, table, bs))
+        results.append(out)
+        del kc, vc
+    assert ops.read_status() == 0
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    torch.cuda.empty_cache()

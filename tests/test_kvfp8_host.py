@@ -101,6 +101,7 @@ def test_decode_refusals():
     _err(_decode(bs=96), _lib.ERR_UNSUPPORTED, "multiple of 64")
     _err(_decode(stride=63), _lib.ERR_INVALID, "geometry")
     _err(_decode(batch=70000), _lib.ERR_UNSUPPORTED, "65535")
+    _err(_decode(width=(1 << 24) + 1, stride=1 << 25), _lib.ERR_UNSUPPORTED, "2^30 keys")
     _err(_decode(), _lib.ERR_WORKSPACE, "workspace")
     _err(_decode(ws=ctypes.c_void_p(0x10010), wsb=1 << 30), _lib.ERR_INVALID, "256-byte")
 

@@ -36,6 +36,7 @@ def test_c_refusals():
                            (dict(q=ODD), _lib.ERR_UNSUPPORTED, b"16-byte multiples"),
                            (dict(qstride=1020), _lib.ERR_UNSUPPORTED, b"16-byte multiples"),
                            (dict(batch=70000), _lib.ERR_UNSUPPORTED, b"65535"),
+                           (dict(width=1 << 24), _lib.ERR_UNSUPPORTED, b"2^30 keys"),
                            (dict(ws=None), _lib.ERR_WORKSPACE, b"workspace"),
                            (dict(wsb=16), _lib.ERR_WORKSPACE, b"workspace"),
                            (dict(ws=ODD), _lib.ERR_INVALID, b"256-byte")):
