@@ -45,7 +45,10 @@
 // Shared mode (decode over a prefix that a whole batch shares,
 // shared_prefix.cu): the batch's rows are one sequence's query tokens, every
 // key of the prefix is visible to all of them, no tile is partial, and every
-// CTA writes fp32 partials of its split of the keys.
+// CTA writes fp32 partials of its split of the keys. Tensor- and softmax-bound
+// like the prefill: 2.2 us a tile of 256 rows x 128 keys, and about 11 us to
+// start and to write the partials (16,384 keys, 512 rows for each of 8 KV heads:
+// 45 us, 0.76 PFLOP/s).
 #include <algorithm>
 #include <cmath>
 #include <mutex>

@@ -14,10 +14,11 @@
 // brought in by a power of two a row, so only elements below 2^-14 of the
 // row's largest lose bits (2^-25 of it).
 //
-// HBM-bound: 258 bytes a (key, KV head) against 4 * 128 * group flops. What is
-// left to hide is the arithmetic around the products, so the keys are the M
-// rows of the MMAs and the query heads the 8 columns (S^T = K Q^T, O^T =
-// V^T W^T): with up to 8 heads a group no MMA row and no softmax lane is
+// HBM-bound: 258 bytes a (key, KV head) against 4 * 128 * group flops (256
+// sequences of 100 to 2048 keys, 16/8 heads: 88 us, 6.1 TB/s, 0.93 of a copy's
+// rate; 32 sequences of 4k to 32k keys, 64/8 heads: 177 us, 6.0 TB/s). What is
+// left to hide is the arithmetic around the products, so the keys are the M rows
+// of the MMAs and the query heads the 8 columns (S^T = K Q^T, O^T = V^T W^T): with up to 8 heads a group no MMA row and no softmax lane is
 // padding, and the conversions (2 a 4-byte word, plus one byte permute for V)
 // serve all heads. A warp owns whole 64-key tiles, the warps of a CTA taking
 // turns, so maxima, barrier waits and rescales are paid once for 64 keys. Each
@@ -568,11 +569,15 @@ int launch_merge_partials(const DecodeParams& p, const float* first_o, const flo
   const int64_t rows = static_cast<int64_t>(batch) * p.num_heads;
   if (rows > 0x7fffffffLL - kMergeThreads)
     return fail(NVATTN_ERR_INVALID, "decode: too many rows");
-  // Eight warps a row for many partials (131071 keys, 32 of them), and where the
-  // rows then still run at once (80 rows of 12: the call 12.9 -> 11.3 us); one
-  // for many rows of few (6400 rows: 69 us, with eight 80).
-  const bool wide = nfirst + p.nsplit / p.cluster > 16 || rows <= 8 * device_sm_count();
-  const int per_cta = wide ? 1 : kMergeThreads / 32;
+  // Warps a row: eight for many partials (131071 keys, 32 of them); otherwise as
+  // many as have two partials each, while all rows run at once, 64 warps an SM
+  // (2048 rows of up to 15: the call 183 us with one, 179 with four; 80 rows of
+  // 12: 12.9 with one, 11.3 with eight; 6400 rows: 67 with one, 69 with two).
+  const int parts = nfirst + p.nsplit / p.cluster;
+  const int64_t room = 64 * static_cast<int64_t>(device_sm_count());
+  int w = 1;
+  while (w < kMergeThreads / 32 && (parts > 16 || (parts >= 2 * w && rows * 2 * w <= room))) w *= 2;
+  const int per_cta = kMergeThreads / 32 / w;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta));
   cfg.blockDim = dim3(kMergeThreads);
@@ -582,11 +587,12 @@ int launch_merge_partials(const DecodeParams& p, const float* first_o, const flo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  const auto kernel = w == 8   ? merge_partials_kernel<8>
+                      : w == 4 ? merge_partials_kernel<4>
+                      : w == 2 ? merge_partials_kernel<2>
+                               : merge_partials_kernel<1>;
   const cudaError_t e =
-      wide ? cudaLaunchKernelEx(&cfg, merge_partials_kernel<kMergeThreads / 32>, p, first_o,
-                                first_ml, nfirst, static_cast<int>(rows))
-           : cudaLaunchKernelEx(&cfg, merge_partials_kernel<1>, p, first_o, first_ml, nfirst,
-                                static_cast<int>(rows));
+      cudaLaunchKernelEx(&cfg, kernel, p, first_o, first_ml, nfirst, static_cast<int>(rows));
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "merge_partials launch");
 }
 

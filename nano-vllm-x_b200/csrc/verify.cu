@@ -23,10 +23,14 @@
 // against its own maximum) and one cluster barrier: every warp writes its sums
 // into the shared memory of all CTAs, and after the barrier every warp adds the
 // same numbers up and takes the same decision, with nothing to broadcast. Rows
-// are a chain, bound by latency (about 5 us a node): the next node's rows are
-// sent for to L2 before it is accepted, and the code of a step is kept short
-// (it once overran the instruction cache at twice the time). The draw then goes
-// over each sequence's last row, all sequences at once.
+// are a chain, bound by latency (about 5 us a node alone, 7 beside 63 other
+// sequences): the next node's rows are sent for to L2 before it is accepted, and
+// the code of a step is kept short (it once overran the instruction cache at
+// twice the time). The draw then goes over each sequence's last row, all
+// sequences at once. 64 sequences of 7 drafts, 151,936 columns: walk 75 us, draw
+// 46; both in one kernel, where an early end is drawn at once, take the same 120,
+// and so does a step that sums up a node's and its first child's rows together
+// (130) or a table of weights over the rows' bf16 values for the draw (121).
 //
 // The answers are tokens, so sums that decide between neighbours are kept in
 // 64 bits: the draw's cumulative weights always (with 151,936 weights of which
