@@ -303,8 +303,8 @@ NVATTN_API int nvattn_paged_decode_fp8(
  * sequences have in common read and multiplied once for the whole batch.
  *
  * Their pages are the first shared_len / block_size entries of row 0 of
- * block_table (rows with at least shared_len keys are taken to hold the same
- * ids there); key j >= shared_len of sequence b comes through row b.
+ * block_table, whatever that row's own length (rows with at least shared_len
+ * keys are taken to hold the same ids there); key j >= shared_len of sequence b comes through row b.
  * cache_seqlens counts all keys of a sequence; a row with fewer than
  * shared_len keys (0: a padding row, whose output is zeros) is attended over
  * its own pages alone. shared_len is a multiple of block_size (0: none shared),

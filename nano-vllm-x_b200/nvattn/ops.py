@@ -197,6 +197,11 @@ def _check_table(block_table: torch.Tensor, rows: int) -> None:
         raise ValueError("block_table rows must be contiguous")
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """t.stride(0), which torch leaves at any value where there is one row."""
+    return t.stride(0) if t.shape[0] != 1 else t.shape[1] * t.stride(1)
+
+
 def _check_decode(q: torch.Tensor, out: torch.Tensor | None, cache_seqlens: torch.Tensor,
                   block_table: torch.Tensor, num_kv_heads: int, cache_dim: int):
     """Argument checks of the decode operators; returns (batch, heads, d, out)."""
@@ -501,7 +506,7 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     with _on_device(dev):
         _lib.call("nvattn_load_kvcache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
                   k_scale.data_ptr(), v_scale.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs,
-                  block_table.data_ptr(), block_table.stride(0), block_table.shape[1], num_blocks,
+                  block_table.data_ptr(), _row_stride(block_table), block_table.shape[1], num_blocks,
                   block_size, num_kv_heads, d, total_k, 1 if new else 0, k_out.data_ptr(),
                   v_out.data_ptr(), *_launch_args(dev))
     return k_out, v_out
@@ -532,10 +537,10 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         ws_ptr, ws_bytes, _ws = _workspace(
             decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size),
             workspace, q)
-        _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), q.stride(0), q.stride(1),
+        _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), _row_stride(q), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),
-                  block_table.data_ptr(), block_table.stride(0), max_blocks, num_blocks,
+                  block_table.data_ptr(), _row_stride(block_table), max_blocks, num_blocks,
                   block_size, batch, num_heads, num_kv_heads, head_dim,
                   head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
                   ws_bytes, *_launch_args(dev))
@@ -558,8 +563,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """``paged_decode`` for a batch whose sequences share their first ``shared_len`` keys.
 
     The shared pages are the first shared_len / block_size entries of row 0 of
-    block_table, read once for the whole batch; keys behind them come through
-    each sequence's own row. cache_seqlens counts all keys; a row with fewer
+    block_table (whatever row 0's own length), read once for the whole batch; keys
+    behind them come through each sequence's own row. cache_seqlens counts all keys; a row with fewer
     than shared_len (0: padding, zeros) is attended over its own row alone.
     shared_len must be whole blocks, block_size a multiple of 128. With
     k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
@@ -587,11 +592,11 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         ws_ptr, ws_bytes, _ws = _workspace(
             shared_prefix_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size,
                                           shared_len, fp8), workspace, q)
-        _lib.call("nvattn_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1),
+        _lib.call("nvattn_shared_prefix_decode", q.data_ptr(), _row_stride(q), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if fp8 else None,
                   v_scale.data_ptr() if fp8 else None, out.data_ptr(), out.stride(0),
                   out.stride(1), cache_seqlens.data_ptr(), block_table.data_ptr(),
-                  block_table.stride(0), max_blocks, num_blocks, block_size, shared_len, batch,
+                  _row_stride(block_table), max_blocks, num_blocks, block_size, shared_len, batch,
                   num_heads, num_kv_heads, head_dim,
                   head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), ws_ptr,
                   ws_bytes, *_launch_args(dev))

@@ -484,3 +484,23 @@ def test_load_of_no_sequences_gives_zeros():
     none = torch.zeros(1, dtype=torch.int32, device=dev)
     k, v = ops.load_kvcache_fp8(kc, kc, ks, ks, none, none.new_empty(0, 4), 5)
     assert k.shape == (5, 3, 128) and not k.any() and not v.any()
+
+
+def test_single_rows_whose_strides_are_arbitrary():
+    """One sequence: torch leaves the stride of a dimension of size one at any value."""
+    H, kvh, bs, n = 4, 2, 128, 300
+    g = torch.Generator().manual_seed(91)
+    (kc, ks), (vc, vs) = [filled_cache(4, bs, kvh, g) for _ in "kv"]
+    q = torch.randn(1, H, 128, generator=g).to(torch.bfloat16)
+    bt = torch.tensor([[3, 1, 0]], dtype=torch.int32)
+    ref, mag = R.decode_attention_f64(q, R.expand_cache_fp8(kc, ks), R.expand_cache_fp8(vc, vs), [n], bt,
+                                      SCALE)
+    odd_q = torch.as_strided(q.to(dev), (1, H, 128), (3, 128, 1))
+    odd_bt = torch.as_strided(bt.to(dev), (1, 3), (1, 1))
+    c = [t.to(dev) for t in (kc, vc, ks, vs)]
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    check(ops.paged_decode_fp8(odd_q, *c, lens, odd_bt, softmax_scale=SCALE), ref, mag, "one row")
+    out = ops.shared_prefix_decode(odd_q, c[0], c[1], lens, odd_bt, bs, SCALE, c[2], c[3])
+    assert (out.double().cpu() - ref).abs().max() <= 1e-2 + 2.0 ** -8 * ref.abs().max()
+    k, _ = ops.load_kvcache_fp8(*c, cu([n]).to(dev), odd_bt, n)
+    assert torch.equal(k[:bs].double().cpu(), R.expand_cache_fp8(kc, ks)[3])
