@@ -33,6 +33,7 @@ allocator, so the decode path can be captured in a CUDA graph the way
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -220,10 +221,17 @@ def _check_decode(q: torch.Tensor, out: torch.Tensor | None, cache_seqlens: torc
     if cache_seqlens.numel() != batch:
         raise ValueError("cache_seqlens must have one entry per row of q")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.stride(2) != 1:
         raise ValueError("out must have q's shape and a contiguous last dimension")
     return batch, num_heads, head_dim, out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, entry: str, *sizes: int) -> int:
+    """A workspace size by the library's own policy, asked for once per sizes and device (the
+    policy looks at the current device, which the callers have made `device`)."""
+    return int(getattr(_lib.load(), entry)(*sizes))
 
 
 def _workspace(need: int, workspace: torch.Tensor | None, like: torch.Tensor):
@@ -535,8 +543,8 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     max_blocks = block_table.shape[1]
     with _on_device(dev):
         ws_ptr, ws_bytes, _ws = _workspace(
-            decode_fp8_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size),
-            workspace, q)
+            _workspace_bytes(dev, "nvattn_decode_fp8_workspace_bytes", batch, num_heads,
+                             num_kv_heads, max_blocks, block_size), workspace, q)
         _lib.call("nvattn_paged_decode_fp8", q.data_ptr(), _row_stride(q), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   out.data_ptr(), out.stride(0), out.stride(1), cache_seqlens.data_ptr(),
@@ -590,8 +598,9 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     shared_len, max_blocks = int(shared_len), block_table.shape[1]
     with _on_device(dev):
         ws_ptr, ws_bytes, _ws = _workspace(
-            shared_prefix_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size,
-                                          shared_len, fp8), workspace, q)
+            _workspace_bytes(dev, "nvattn_shared_prefix_workspace_bytes", batch, num_heads,
+                             num_kv_heads, max_blocks, block_size, shared_len, int(fp8)),
+            workspace, q)
         _lib.call("nvattn_shared_prefix_decode", q.data_ptr(), _row_stride(q), q.stride(1),
                   k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if fp8 else None,
                   v_scale.data_ptr() if fp8 else None, out.data_ptr(), out.stride(0),
