@@ -214,12 +214,14 @@ __device__ __forceinline__ uint64_t exp2_mufu_f32x2(uint64_t x2) {
 // x = n + f with n = round(x) (adding 1.5*2^23 leaves n in the low mantissa
 // bits), f in [-0.5, 0.5]; 2^f from a cubic fitted here to relative error
 // 7.5e-5 (near-minimax: Lawson-weighted least squares on Chebyshev nodes),
-// then n is added to the exponent field. Inputs are clamped to >= -127
-// (result ~6e-39, i.e. zero for a softmax sum that is >= 2^-8).
+// then n is added to the exponent field. Inputs are clamped to >= -126
+// (result ~1.2e-38, i.e. zero for a softmax sum that is >= 2^-8). Not below: the
+// cubic at f = 0 is just under 1, exponent field 126, and n = -127 would carry
+// into the sign, a NaN.
 __device__ __forceinline__ uint64_t exp2_poly_f32x2(uint64_t x2) {
   float2 x = unpack_f32x2(x2);
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
   const uint64_t xc = pack_f32x2(x.x, x.y);
   const uint64_t t = add_f32x2(xc, pack_f32x2(12582912.f, 12582912.f));
   const uint64_t n = add_f32x2(t, pack_f32x2(-12582912.f, -12582912.f));
