@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
           break;
         }
         const int tok0 = tok_begin + it * kTile;
-        int blk = bt[tok0 / p.block_size];
+        int blk = kSuffix ? page_of(p, bt, tok0, ctx) : bt[tok0 / p.block_size];
         if (blk < 0 || blk >= p.num_blocks) {
           set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
           blk = 0;  // read a valid block; the result is flagged as invalid
@@ -558,6 +558,7 @@ extern "C" int nvattn_paged_decode(const void* q, int64_t q_stride_tok, int64_t 
   p.split_tiles = split_tiles;
   p.cluster = 1;
   p.key_begin = 0;
+  p.shared = 0;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);

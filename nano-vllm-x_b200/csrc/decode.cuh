@@ -29,6 +29,7 @@ struct DecodeParams {
   int32_t nsplit, split_tiles;
   int32_t cluster;   // fp8: splits that one cluster merges before it writes (divides nsplit)
   int32_t key_begin;  // suffix kernels: first key of the split range (a whole number of blocks)
+  int32_t shared;  // keys whose pages row 0 of the table holds, for rows with at least as many (0: none)
   float scale_log2;
   float* ws_o;    // [batch][num_heads][nsplit][128]
   float2* ws_ml;  // [batch][num_heads][nsplit]  (running max (log2 units), sum)
@@ -58,6 +59,11 @@ __device__ __forceinline__ void join_prefix_grid() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The table entry of key `tok` of a row with ctx keys.
+__device__ __forceinline__ int page_of(const DecodeParams& p, const int32_t* row, int tok, int ctx) {
+  return __ldg((tok < p.shared && ctx >= p.shared ? p.block_table : row) + tok / p.block_size);
+}
+
 // Split size for a batch over tables of max_blocks, of at least min_tiles (see
 // decode.cu).
 constexpr int kMinSplitTiles = NVATTN_DEC_MIN_SPLIT_TILES;
@@ -84,6 +90,10 @@ int check_decode_args(const char* who, const void* q, int64_t q_stride_tok, int6
 // dependents of the prefix's kernel, launched just before on `stream`.
 int launch_decode_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache, int batch,
                          bool after_prefix, cudaStream_t stream);
+// All keys of every row, merged into p.out.
+int launch_decode_fp8_whole(const DecodeParams& p, const void* k_cache, const void* v_cache,
+                            const uint8_t* k_scale, const uint8_t* v_scale, int batch,
+                            cudaStream_t stream);
 int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
                              bool after_prefix, cudaStream_t stream);

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(dec8_warps(NB) * 32, dec8_ctas(NB))
   const int32_t* bt = p.block_table + static_cast<int64_t>(b) * p.bt_stride;
   auto page = [&](int it) {
     if (it >= ntiles) return 0;
-    const int blk = bt[(tok_begin + it * kTile) / p.block_size];
+    const int blk = page_of(p, bt, tok_begin + it * kTile, ctx);
     if (blk >= 0 && blk < p.num_blocks) return blk;
     set_status(p.status, NVATTN_STATUS_BAD_BLOCK);
     return 0;  // read a valid block; the result is flagged as invalid
@@ -651,6 +651,17 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode_fp8 launch");
 }
 
+int launch_decode_fp8_whole(const DecodeParams& p, const void* k_cache, const void* v_cache,
+                            const uint8_t* k_scale, const uint8_t* v_scale, int batch,
+                            cudaStream_t stream) {
+  const int rc = p.group <= 8 ? launch_decode_fp8<1, false>(p, k_cache, v_cache, k_scale, v_scale,
+                                                            batch, false, stream)
+                              : launch_decode_fp8<2, false>(p, k_cache, v_cache, k_scale, v_scale,
+                                                            batch, false, stream);
+  if (rc || p.nsplit == p.cluster) return rc;
+  return launch_merge_partials(p, nullptr, nullptr, 0, batch, stream);
+}
+
 int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
                              bool after_prefix, cudaStream_t stream) {
@@ -764,10 +775,6 @@ extern "C" int nvattn_paged_decode_fp8(
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(NVATTN_ERR_INVALID, "paged_decode_fp8: workspace must be 256-byte aligned");
   set_decode_workspace(&p, need > 0 ? workspace : nullptr, batch);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  rc = p.group <= 8
-           ? launch_decode_fp8<1, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s)
-           : launch_decode_fp8<2, false>(p, k_cache, v_cache, k_scale, v_scale, batch, false, s);
-  if (rc || p.nsplit == p.cluster) return rc;
-  return launch_merge_partials(p, nullptr, nullptr, 0, batch, s);
+  return launch_decode_fp8_whole(p, k_cache, v_cache, k_scale, v_scale, batch,
+                                 reinterpret_cast<cudaStream_t>(stream));
 }

@@ -10,7 +10,8 @@
 // over P * kv_heads * 512 bytes: tensor-bound from a few hundred rows on). The
 // own keys are the split-K decode kernels (decode.cu, decode_fp8.cu), bound by
 // HBM, launched to run beside the prefix's last CTAs; a last kernel merges the
-// fp32 partials of both. With an fp8 cache the prefix is expanded to bf16 in
+// fp32 partials of both. Short prefixes of few rows are read once a row instead
+// (prefix_apart below). With an fp8 cache the prefix is expanded to bf16 in
 // the workspace first: it is read once by that, and the tensor-core kernel
 // takes it from L2.
 #include <algorithm>
@@ -24,25 +25,39 @@ static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255);
 
 // Byte offsets of the workspace's regions and the splits they hold.
 struct SharedLayout {
-  int np, ptiles;  // splits of the prefix (0: no prefix)
+  int np, ptiles;  // splits of the prefix (0: none, or read with the own keys)
   int ns, stiles, cluster;  // splits of the own keys; those that a cluster merges
   size_t prefix_o, prefix_ml, own, k, v, bytes;
 };
 
+// The prefix is attended apart from the own keys where reading it once a row
+// would cost more than the extra launches and partials: from 32 MB of such reads
+// on (bf16; 16/8 heads, 5 rows of 1024: 11.8 us apart, 9.6 in one; 8 rows of 1024,
+// 32 MB: 12.6 and 12.7; 8 rows of 2048: 15.5 and 16.3; 32/8 heads, 32 rows of 512,
+// 64 MB: 15.7 and 21.2), with an fp8 cache, whose prefix is expanded first, from
+// 64 MB on (16 rows of 1024, 32 MB: 17.7 and 11.9; 32/8 heads, 32 rows of 1024, 64
+// MB: 20.4 and 20.3; 64 rows of 1024: 25.3 and 32.8). Otherwise the decode kernel
+// takes all keys of a row, the shared pages from row 0 of the table.
+static bool prefix_apart(int batch, int num_kv_heads, int shared_len, bool fp8) {
+  const int64_t keys = static_cast<int64_t>(batch) * shared_len * num_kv_heads;
+  return fp8 ? keys * 258 > (64 << 20) : keys * 512 > (32 << 20);
+}
+
 static SharedLayout shared_layout(int batch, int num_heads, int num_kv_heads, int max_blocks,
                                   int block_size, int shared_len, bool fp8) {
   SharedLayout w{};
-  if (shared_len > 0)
-    shared_split(batch, num_heads, num_kv_heads, shared_len, &w.np, &w.ptiles);
-  const int own_blocks = std::max(1, max_blocks - shared_len / block_size);
+  const bool apart = prefix_apart(batch, num_kv_heads, shared_len, fp8);
+  if (apart) shared_split(batch, num_heads, num_kv_heads, shared_len, &w.np, &w.ptiles);
+  const int own_blocks = std::max(1, max_blocks - (apart ? shared_len / block_size : 0));
   w.cluster = 1;
   if (fp8)
     choose_split_fp8(batch, num_kv_heads, static_cast<int64_t>(own_blocks) * block_size, &w.ns,
                      &w.stiles, &w.cluster);
   else
-    // the merge runs anyway: splits of 8 tiles (64 rows x 8 KV heads of up to 1023
+    // behind a prefix: splits of 8 tiles (64 rows x 8 KV heads of up to 1023
     // own keys 75 us the call, of 4 tiles 79, of 16 76)
-    choose_split(batch, num_kv_heads, own_blocks, block_size, &w.ns, &w.stiles, 8);
+    choose_split(batch, num_kv_heads, own_blocks, block_size, &w.ns, &w.stiles,
+                 apart ? 8 : kMinSplitTiles);
   const size_t rows = static_cast<size_t>(batch) * num_heads;
   size_t at = 0;
   w.prefix_o = at;
@@ -52,7 +67,7 @@ static SharedLayout shared_layout(int batch, int num_heads, int num_kv_heads, in
   w.own = at;
   const size_t parts = rows * (w.ns / w.cluster);
   at += round256(parts * kHeadDim * sizeof(float)) + round256(parts * sizeof(float2));
-  if (fp8) {
+  if (fp8 && apart) {
     const size_t kv = static_cast<size_t>(shared_len) * num_kv_heads * kHeadDim * 2;
     w.k = at;
     at += round256(kv);
@@ -140,7 +155,8 @@ extern "C" int nvattn_shared_prefix_decode(
   p.nsplit = w.ns;
   p.split_tiles = w.stiles;
   p.cluster = w.cluster;
-  p.key_begin = shared_len;
+  p.key_begin = w.np > 0 ? shared_len : 0;
+  p.shared = w.np > 0 ? 0 : shared_len;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = status;
   set_decode_workspace(&p, ws + w.own, batch);
@@ -183,6 +199,8 @@ extern "C" int nvattn_shared_prefix_decode(
     if (rc) return rc;
   }
   const bool after = w.np > 0;
+  if (fp8 && !after)
+    return launch_decode_fp8_whole(p, k_cache, v_cache, k_scale, v_scale, batch, s);
   rc = fp8 ? launch_decode_fp8_suffix(p, k_cache, v_cache, k_scale, v_scale, batch, after, s)
            : launch_decode_suffix(p, k_cache, v_cache, batch, after, s);
   if (rc) return rc;

@@ -87,6 +87,13 @@ def run(q, caches, scales, lens, bt, shared, **kw):
                                     v_scale=to(scales[1]), **kw)
 
 
+def apart(lens, kvh, shared, fp8):
+    """Padding rows that bring a batch past the size from which the prefix is attended apart from
+    the own keys: 32 MB of K and V read once a row (64 MB in fp8)."""
+    need = (64 << 20) // (258 * kvh * shared) if fp8 else (32 << 20) // (512 * kvh * shared)
+    return list(lens) + [0] * max(0, need + 1 - len(lens))
+
+
 def case(B, H, kvh, bs, shared, lens, fp8, seed=0, **kw):
     caches, scales, vals, bt = build(B, kvh, bs, shared, lens, fp8, seed, **kw)
     q = torch.randn(B, H, 128, generator=torch.Generator().manual_seed(seed + 1)).to(torch.bfloat16)
@@ -104,7 +111,10 @@ def case(B, H, kvh, bs, shared, lens, fp8, seed=0, **kw):
                                                (70, 8, 2, 128, 1280), (9, 24, 2, 512, 1024)])
 def test_equals_64_bits(B, H, kvh, bs, shared, fp8):
     own = np.random.default_rng(B).integers(1, 400, size=B)
-    case(B, H, kvh, bs, shared, (shared + own).tolist(), fp8, seed=B)
+    lens = (shared + own).tolist()
+    case(B, H, kvh, bs, shared, lens, fp8, seed=B)
+    lens = apart(lens, kvh, shared, fp8)
+    case(len(lens), H, kvh, bs, shared, lens, fp8, seed=B)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -112,16 +122,21 @@ def test_own_lengths_around_tiles_and_short_rows(fp8):
     """No own key, one, tile edges; padding rows; rows with fewer keys than the prefix."""
     shared = 512
     lens = [shared + n for n in (1, 0, 63, 64, 65, 127, 128, 129, 300)] + [0, 1, 64, 511, 0, 200]
-    out = case(len(lens), 8, 2, 128, shared, lens, fp8, seed=7)
-    assert (out[9] == 0).all() and (out[13] == 0).all()
+    for lens in (lens, apart(lens, 2, shared, fp8)):
+        out = case(len(lens), 8, 2, 128, shared, lens, fp8, seed=7)
+        assert (out[9] == 0).all() and (out[13] == 0).all() and (out[15:] == 0).all()
 
 
 @pytest.mark.parametrize("fp8", [False, True])
 def test_no_row_has_own_keys_or_none_reaches_the_prefix(fp8):
-    case(4, 4, 2, 128, 256, [256] * 4, fp8, seed=8)           # the table ends with the prefix
-    case(3, 4, 2, 128, 1024, [5, 700, 0], fp8, seed=9)         # all shorter
-    out = case(3, 4, 2, 128, 256, [0, 0, 0], fp8, seed=10)
-    assert (out == 0).all()
+    for pad in (lambda lens, *_: lens, apart):
+        lens = pad([256] * 4, 2, 256, fp8)
+        case(len(lens), 4, 2, 128, 256, lens, fp8, seed=8)     # the table ends with the prefix
+        lens = pad([5, 700, 0], 2, 1024, fp8)
+        case(len(lens), 4, 2, 128, 1024, lens, fp8, seed=9)    # all shorter
+        lens = pad([0, 0, 0], 2, 256, fp8)
+        out = case(len(lens), 4, 2, 128, 256, lens, fp8, seed=10)
+        assert (out == 0).all()
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -137,7 +152,7 @@ def test_wide_table_and_long_prefix():
 
 def test_growing_maxima_in_the_prefix():
     """Keys scaled up deep in the prefix: every row's maximum grows far past the rescale threshold."""
-    B, H, kvh, bs, shared = 40, 4, 1, 128, 1024
+    B, H, kvh, bs, shared = 80, 4, 1, 128, 1024  # attended apart
     lens = [shared + 50] * B
     caches, scales, vals, bt = build(B, kvh, bs, shared, lens, False, 14)
     for page, mul in ((int(bt[0, 3]), 6.0), (int(bt[0, 6]), 14.0)):
@@ -149,11 +164,14 @@ def test_growing_maxima_in_the_prefix():
     check(out, ref, mag, "growing maxima")
 
 
-def test_agrees_with_paged_decode():
-    lens = [600, 513, 900, 0, 512]
+@pytest.mark.parametrize("pad", [False, True])
+def test_agrees_with_paged_decode(pad):
     for fp8 in (False, True):
-        caches, scales, _, bt = build(5, 2, 128, 512, lens, fp8, 15)
-        q = torch.randn(5, 8, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+        lens = [600, 513, 900, 0, 512]
+        if pad:
+            lens = apart(lens, 2, 512, fp8)
+        caches, scales, _, bt = build(len(lens), 2, 128, 512, lens, fp8, 15)
+        q = torch.randn(len(lens), 8, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
         a = run(q, caches, scales, lens, bt, 512)
         sl = torch.tensor(lens, dtype=torch.int32, device=dev)
         if fp8:
@@ -164,17 +182,18 @@ def test_agrees_with_paged_decode():
         assert (a.float() - b.float()).abs().max() < 4 * 2.0 ** -8 * 3
 
 
-def test_bad_pages_and_lengths_are_flagged():
-    lens = [300, 300]
-    caches, scales, _, bt = build(2, 1, 128, 256, lens, False, 16)
-    q = torch.randn(2, 2, 128).to(torch.bfloat16)
+@pytest.mark.parametrize("pad", [False, True])
+def test_bad_pages_and_lengths_are_flagged(pad):
+    lens = apart([300, 300], 1, 256, False) if pad else [300, 300]
+    caches, scales, _, bt = build(len(lens), 1, 128, 256, lens, False, 16)
+    q = torch.randn(len(lens), 2, 128).to(torch.bfloat16)
     for where, value in (((0, 1), 1000), ((0, 1), -5), ((1, 2), 77)):
         bad = bt.clone()
         bad[where] = value
         ops.read_status()
         run(q, caches, scales, lens, bad, 256)
         assert ops.read_status() == nvattn._lib.STATUS_BAD_BLOCK
-    run(q, caches, scales, [300, 128 * bt.shape[1] + 1], bt, 256)
+    run(q, caches, scales, [300, 128 * bt.shape[1] + 1] + lens[2:], bt, 256)
     assert ops.read_status() == nvattn._lib.STATUS_BAD_BLOCK
 
 
@@ -195,11 +214,29 @@ def test_strided_q_and_out_and_checks():
         run(qkv[:, :512].view(2, 4, 128), caches, scales, lens, bt, 200)
 
 
+def test_only_row_0_of_the_table_holds_the_prefix():
+    """The other rows' entries for it are not read, unless the row is shorter than the prefix."""
+    for fp8 in (False, True):
+        for pad in (False, True):
+            lens = [600, 700, 300, 512, 1]
+            if pad:
+                lens = apart(lens, 2, 512, fp8)
+            caches, scales, vals, bt = build(len(lens), 2, 128, 512, lens, fp8, 19)
+            q = torch.randn(len(lens), 8, 128, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+            ref, mag = R.decode_attention_f64(q, *vals, lens, bt.clamp_min(0), SCALE)
+            bt[1, :4] = bt[3, :4] = -1
+            ops.read_status()
+            check(run(q, caches, scales, lens, bt, 512), ref, mag, "row 0")
+            assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("B", [10, 260])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_graphs_and_streams(fp8):
-    """Two captured graphs with pools of their own and eager calls on two streams at once."""
-    B, H, kvh, bs, shared, width = 10, 8, 2, 128, 512, 8
-    lens = [900] * B
+def test_graphs_and_streams(fp8, B):
+    """Two captured graphs with pools of their own and eager calls on two streams at once, of a
+    batch that reads the prefix with its own keys and of one (mostly padding) that does not."""
+    H, kvh, bs, shared, width = 8, 2, 128, 512, 8
+    lens = [900] * 10 + [0] * (B - 10)
     caches, scales, vals, bt = build(B, kvh, bs, shared, lens, fp8, 18, width=width, stale=False)
     args = [t.to(dev) for t in caches]
     sc = dict(k_scale=None, v_scale=None)
@@ -222,6 +259,7 @@ def test_graphs_and_streams(fp8):
     for trial in range(2):
         new = np.random.default_rng(trial).integers(shared, 900, size=B)
         new[-2:] = 0
+        new[10:] = 0
         qn = torch.randn(B, H, 128, generator=g).to(torch.bfloat16)
         q.copy_(qn), sl.copy_(torch.from_numpy(new.astype(np.int32)))
         for graph, _ in graphs:

@@ -48,8 +48,10 @@ def test_workspace_depends_on_host_sizes():
     slot = 128 * 4 + 8
     # nothing shared: the own keys' partials, one split at least
     assert f(4, 8, 2, 1, 128, 0) >= 4 * 8 * slot
-    # an fp8 prefix adds its bf16 rows
-    assert f(4, 8, 2, 9, 128, 1024, True) - f(4, 8, 2, 9, 128, 1024) == 2 * 1024 * 2 * 128 * 2
+    # an fp8 prefix that is attended apart adds its bf16 rows
+    assert f(200, 8, 2, 9, 128, 1024, True) - f(200, 8, 2, 9, 128, 1024) == 2 * 1024 * 2 * 128 * 2
+    # a short one of few rows is read with the own keys: no partials of its own
+    assert f(4, 8, 2, 9, 128, 1024) < f(100, 8, 2, 9, 128, 1024) // 25
     # sizes that the call refuses need no workspace
     assert f(4, 8, 2, 9, 128, 100) == 0 and f(0, 8, 2, 9, 128, 128) == 0
     assert f(4, 8, 3, 9, 128, 128) == 0 and f(4, 8, 2, 9, 128, 10 * 128) == 0
