@@ -130,8 +130,9 @@ __device__ __forceinline__ void fill_table(double* table) {
 
 // One row's scale in fp64: the weight of a bf16 logit l is 2^((l - top) * c),
 // held above 2^-1000 (no draw reaches weights below kNothing). c is at most what
-// puts the next bf16 below the top at 2^-2000, so that top * c stays small
-// enough for its rounding. Rows whose largest logit is infinite are weighed as 0
+// puts the next bf16 below the top at 2^-2000, and has 45 significant bits
+// (changing a weight by 2^-45 of its exponent), so that l * c and top * c are
+// exact: the exponent is rounded once, and the top's weight is one. Rows whose largest logit is infinite are weighed as 0
 // for an infinite logit and -980 for any other, with c = 1.
 struct RowScale {
   double c, top_c;
@@ -145,6 +146,7 @@ struct RowScale {
                                                       : top_bits - 1u;
     const double gap = static_cast<double>(top) - static_cast<double>(__uint_as_float(below << 16));
     c = inf ? 1.0 : (c64 * gap > 2000.0 ? 2000.0 / gap : c64);
+    c = __longlong_as_double(__double_as_longlong(c) & ~0xffll);
     top_c = inf ? 0.0 : static_cast<double>(top) * c;
   }
   // NaN and -inf become the lowest bf16.
@@ -716,7 +718,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   const int len = min(p.slice, p.vocab - x0);
   const double c64 = 1.4426950408889634074 / static_cast<double>(temp);
   const RowScale scale(st.top, c64), qscale(st.qtop == kNoLogit ? 0u : st.qtop, c64);
-  const double ratio = static_cast<double>(st.ratio);
+  double ratio = static_cast<double>(st.ratio);
   bool use_q = kDraft && st.qtop != kNoLogit;
   const Slice ps(row_of(p.logits, b, p.l_stride_seq, node, p.l_stride_row) + x0, len);
   const Slice qs(
@@ -783,12 +785,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   };
 
   double pinv = 1.0, qinv = 0.0;
+  bool exact = false, again = false;  // ratio is that of the exact sums; a second draw, from p
 #pragma unroll 1
-  for (int attempt = 0;; ++attempt) {
+  while (true) {
     // ---- one pass. With a draft row it gives the exact sums a, d and, over the
     // columns where p exceeds q by the sums of the walk, the parts ra, rd of the
     // residual: a column on the wrong side by a rounding of those sums has a
-    // residual of no more than that rounding. Otherwise ra is p's.
+    // residual of no more than that rounding (2^-21). Otherwise ra is p's.
     double a = 0.0, d = 0.0, ra = 0.0, rd = 0.0, sa = 0.0, sd = 0.0;
     uint32_t w[4], v[4] = {0u, 0u, 0u, 0u}, wn[4], vn[4];
     issue(group(0), w, v);
@@ -838,8 +841,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
         a += all[i].d.x;
         d += all[i].d.y;
       }
-      pinv = 1.0 / warp_sum(a);
-      qinv = 1.0 / warp_sum(d);
+      a = warp_sum(a);
+      d = warp_sum(d);
+      pinv = 1.0 / a;
+      qinv = 1.0 / d;
       mine = fmax(ra * pinv - rd * qinv, 0.0);
     }
     VerifySlot s;
@@ -852,10 +857,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
       own += lane * each + i < nslots ? all[lane * each + i].d.x : 0.0;
     const double incl = warp_scan(own, lane);
     const double total = __shfl_sync(0xffffffffu, incl, 31);
-    if (!(total > kNothing) && attempt == 0) {
+    if (kDraft && use_q && !exact && !(total > 0x1p-12)) {
+      // rows that almost agree: such roundings would count, so another pass with
+      // the sides by the exact sums
+      ratio = a / d;
+      exact = true;
+      continue;
+    }
+    if (!(total > kNothing) && !again) {
       use_q = skip = false;  // rounding rejected the last of the mass: draw from p
       pinv = 1.0;
       qinv = 0.0;
+      again = true;
       continue;
     }
     const double threshold =

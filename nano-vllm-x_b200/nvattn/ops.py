@@ -505,7 +505,7 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     if new:
         make = k_cache.new_empty if num_seqs else k_cache.new_zeros  # no sequence: all rows zero
         k_out = make(shape, dtype=torch.bfloat16)
-        v_out = make(shape, dtype=torch.bfloat16)
+        v_out = torch.empty_like(k_out) if num_seqs else k_out.clone()
     else:
         _check_bf16(k_out, v_out)
         for n, t in (("k_out", k_out), ("v_out", v_out)):

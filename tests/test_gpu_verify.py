@@ -244,3 +244,41 @@ def test_extreme_temperatures():
                                            1e-45, 2e-4])
         for pv in (0.0, 0.37, 1.0 - 2.0 ** -24):
             _check(x, tok, u, torch.full((12,), pv), kw)
+
+
+@pytest.mark.parametrize("V", [9, 255, 5000])
+@pytest.mark.parametrize("gap", [3.0, 8.0, 16.0, 24.0])
+def test_draft_rows_that_almost_agree(V, gap):
+    """Peaked rows whose residual max(p - q, 0) is small (down to about 1e-10, still far above what 64-bit
+    sums of p and q round off): drafts that q never gives are rejected and the residual drawn from."""
+    g = torch.Generator().manual_seed(int(V + gap))
+    B, n = 48, 4
+    x = torch.randn(B, n, V, generator=g)
+    x.scatter_(2, torch.randint(0, V, (B, n, 1), generator=g), gap)
+    d = x[:, :n - 1].clone()
+    other = torch.randint(0, V, (B, n - 1, 3), generator=g)
+    d.scatter_(2, other, d.gather(2, other) - 1.0)  # the residual: columns that the draft has less of
+    d.scatter_add_(2, other[..., :1].roll(1, 1), torch.full((B, n - 1, 1), 0.5))
+    x, d = x.to(torch.bfloat16), d.to(torch.bfloat16)
+    tok = x[:, :n - 1].float().argmin(-1)
+    tok[:, 0] = x[:, 0].float().argmax(-1)
+    u = torch.full((B, n - 1), 1.0 - 2.0 ** -24)
+    u[:, 0] = 0.5
+    _check(x, tok, u, torch.rand(B, generator=g), dict(temperatures=0.6 + torch.rand(B, generator=g),
+                                                       draft_logits=d))
+
+
+def test_draft_rows_that_agree_but_for_the_deep_tail():
+    """Almost greedy rows with the same largest logit in both: the residual is a single column's weight,
+    100 and more decimal orders below one."""
+    g = torch.Generator().manual_seed(77)
+    B, n, V = 24, 3, 255
+    x = torch.randn(B, n, V, generator=g)
+    d = x[:, :n - 1] + 0.1 * torch.randn(B, n - 1, V, generator=g)
+    top = torch.randint(0, V, (B, 1, 1), generator=g)
+    x.scatter_(2, top.expand(B, n, 1), 4.0 + torch.rand(B, n, 1, generator=g))
+    d.scatter_(2, top.expand(B, n - 1, 1), 4.0 + torch.rand(B, n - 1, 1, generator=g))
+    tok = x[:, :n - 1].float().argmin(-1)
+    _check(x.to(torch.bfloat16), tok, torch.full((B, n - 1), 0.5), torch.rand(B, generator=g),
+           dict(temperatures=torch.full((B,), 4e-3) + 4e-3 * torch.rand(B, generator=g),
+                draft_logits=d.to(torch.bfloat16)))
