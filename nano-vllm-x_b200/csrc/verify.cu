@@ -56,7 +56,7 @@ constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxNodes = 64;
-constexpr int kMaxVocab = 1 << 20;  // keeps the fp32 sums well inside decide()'s margin
+constexpr int kMaxVocab = 1 << 20;  // keeps the fp32 sums well inside the margin of open decisions
 constexpr int kExpTable = 1024;
 constexpr uint32_t kNoLogit = 0xff80u;  // bf16 bits of -inf
 // Temperatures count up to this (every law is flat long before): a logit of
