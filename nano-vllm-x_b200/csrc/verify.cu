@@ -132,28 +132,31 @@ __device__ __forceinline__ void fill_table(double* table) {
 // held above 2^-1000 (no draw reaches weights below kNothing). c is at most what
 // puts the next bf16 below the top at 2^-2000, and has 45 significant bits
 // (changing a weight by 2^-45 of its exponent), so that l * c and top * c are
-// exact: the exponent is rounded once, and the top's weight is one. Rows whose largest logit is infinite are weighed as 0
-// for an infinite logit and -980 for any other, with c = 1.
+// exact: the exponent is rounded once, and the top's weight is one. A row whose top
+// has no finite bf16 below it (infinite, or the lowest finite one) belongs to the
+// logits that equal its top: they are weighed as 0 and any other as -980, with c = 1.
 struct RowScale {
   double c, top_c;
-  bool inf;
+  uint32_t top;  // bf16 bits
+  bool ties;
 
-  __device__ __forceinline__ RowScale(uint32_t top_bits, double c64) {
-    const float top = __uint_as_float(top_bits << 16);
-    inf = top_bits == 0x7f80u;
+  __device__ __forceinline__ RowScale(uint32_t top_bits, double c64) : top(top_bits) {
+    const float top_l = __uint_as_float(top_bits << 16);
+    ties = top_bits == 0x7f80u || top_bits == 0xff7fu;
     const uint32_t below = (top_bits & 0x7fffu) == 0u ? 0x8001u
                            : (top_bits & 0x8000u)     ? top_bits + 1u
                                                       : top_bits - 1u;
-    const double gap = static_cast<double>(top) - static_cast<double>(__uint_as_float(below << 16));
-    c = inf ? 1.0 : (c64 * gap > 2000.0 ? 2000.0 / gap : c64);
+    const double gap =
+        static_cast<double>(top_l) - static_cast<double>(__uint_as_float(below << 16));
+    c = ties ? 1.0 : (c64 * gap > 2000.0 ? 2000.0 / gap : c64);
     c = __longlong_as_double(__double_as_longlong(c) & ~0xffll);
-    top_c = inf ? 0.0 : static_cast<double>(top) * c;
+    top_c = ties ? 0.0 : static_cast<double>(top_l) * c;
   }
-  // NaN and -inf become the lowest bf16.
+  // NaN and -inf become the lowest bf16, which weighs 2^-1000 beside any other top.
   __device__ __forceinline__ uint32_t raise(uint32_t two) const {
-    if (inf)
-      two = ((two & 0xffffu) == 0x7f80u ? 0u : 0xc475u) |
-            ((two >> 16) == 0x7f80u ? 0u : 0xc4750000u);  // -980
+    if (ties)
+      two = ((two & 0xffffu) == top ? 0u : 0xc475u) |
+            ((two >> 16) == top ? 0u : 0xc4750000u);  // -980
     const __nv_bfloat162 lowest(__nv_bfloat162_raw{0xff7fu, 0xff7fu});
     const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&two), lowest);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -930,7 +933,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
       if (pos) lastx = __shfl_sync(0xffffffffu, lx, 31 - __clz(pos));
       sum += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) p.out_tokens[out_row + num] = x0 + (found >= 0 ? found : max(lastx, 0));
+    if (lane == 0)  // weights lie inside the slice
+      p.out_tokens[out_row + num] = x0 + min(max(found >= 0 ? found : lastx, 0), len - 1);
     return;
   }
 }
