@@ -77,6 +77,7 @@ struct VerifyParams {
   const int32_t* num_nodes;    // null: all
   int32_t nodes, vocab, slice;
   int32_t ahead;  // the walk sends for the first child's rows before it is accepted
+  int32_t border;  // near_border, by the walk's batches
   int64_t* out_tokens;
   int32_t* out_path;
   int32_t* out_num;
@@ -180,6 +181,25 @@ __device__ __forceinline__ double exp2_64(double t, const double* __restrict__ t
   const double tj = table[k & (kExpTable - 1)];
   const double r = fma(e * f, tj, tj);
   return __hiloint2double(__double2hiint(r) + ((k & ~(kExpTable - 1)) << 10), __double2loint(r));
+}
+
+// Whether wp may be on the other side of x = wq * ratio by the rows' true sums. The
+// ratio is that of the walk's sums, in fp32: a thread takes 40 columns at a time (12
+// additions; exp2 is off by 2^-22.5, its argument, in a row of 2^20 columns, by 2e-6
+// of the terms that count), scales and adds once a batch (3.3e-7), and then come 20
+// additions and scalings over threads, warps and CTAs: 4.5e-6 and 3.3e-7 a batch at
+// most, twice that for the quotient. That is 1.5e-5 with kShortBatches and 4.4e-5 with
+// the most there are (kMaxVocab columns on 512 threads, 53 batches). `border` is 1.5 *
+// 2^-16 or 2^-14 of a mantissa of up to 2 in steps of 2^-20, the high words' last bit,
+// and one for the bits below. Weights under 2^-60 are not looked at: all of them
+// together move the residual by less than 2^-53.
+constexpr int kShortBatches = 9, kBorderShort = 49, kBorderLong = 129;
+constexpr int kNears = 8;  // such columns that a thread of the draw notes
+
+__device__ __forceinline__ bool near_border(double wp, double x, int border) {
+  const int hi = __double2hiint(wp);
+  return static_cast<uint32_t>(hi - __double2hiint(x) + border) <= static_cast<uint32_t>(2 * border) &&
+         hi > 0x3C300000;
 }
 
 // Weights up to this count as none: above the sum of all that log2_weight held
@@ -583,8 +603,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_walk_kernel(const Ve
     const bool any = top != kNoLogit, any_q = qtop != kNoLogit;
 
     // ---- which child goes on: every warp of the cluster takes this decision
-    // alike. With the fp32 sums (off by < 2^-17) an outcome within 2^-14 of its
-    // border is left open, and taken again with fp64 sums.
+    // alike. With the fp32 sums (off by 2.2e-5 at most, see near_border) an outcome
+    // within 2^-14 of its border is left open, and taken again with fp64 sums.
     int next = -1;
 #pragma unroll 1
     for (int exact = 0; exact < 2; ++exact) {
@@ -696,6 +716,7 @@ template <bool kDraft>
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const VerifyParams p) {
   __shared__ VerifyShared sh;
   __shared__ double table[kExpTable];
+  __shared__ uint16_t near_at[kDraft ? kNears : 1][kVerifyThreads];  // step * 8 + element
   Exchange exchange(sh);
   const int rank = exchange.rank, ranks = exchange.ranks;
   const int lane = exchange.lane, warp = exchange.warp;
@@ -793,29 +814,38 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   while (true) {
     // ---- one pass. With a draft row it gives the exact sums a, d and, over the
     // columns where p exceeds q by the sums of the walk, the parts ra, rd of the
-    // residual: a column on the wrong side by a rounding of those sums has a
-    // residual of no more than that rounding (2^-21). Otherwise ra is p's.
+    // residual. A thread notes the columns that those sums may have on the wrong
+    // side: of ordinary rows none, a few or, where the rows' logits are on a grid
+    // that meets the border, some hundred of 151,936. Otherwise ra is p's.
     double a = 0.0, d = 0.0, ra = 0.0, rd = 0.0, sa = 0.0, sd = 0.0;
+    int nears = 0;
     uint32_t w[4], v[4] = {0u, 0u, 0u, 0u}, wn[4], vn[4];
     issue(group(0), w, v);
 #pragma unroll 1
     for (int step = 0, in_bin = 0, bin = 0; step < steps; ++step) {
       if (step + 1 < steps) issue(group(step + 1), wn, vn);  // before this step's arithmetic
       finish(group(step), w, v);
+      uint32_t near = 0u;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const double wp = exp2_64(scale.log2_weight(logit(w, e)), table);
         if (kDraft && use_q) {
-          const double wq = exp2_64(qscale.log2_weight(logit(v, e)), table);
+          const double wq = exp2_64(qscale.log2_weight(logit(v, e)), table), x = wq * ratio;
           a += wp;
           d += wq;
-          if (wp > wq * ratio) {
+          if (wp > x) {
             sa += wp;
             sd += wq;
           }
+          near |= static_cast<uint32_t>(near_border(wp, x, p.border)) << e;
         } else {
           sa += wp;
         }
+      }
+      if (kDraft && near) {
+#pragma unroll 1
+        for (; near; near &= near - 1, ++nears)
+          if (nears < kNears) near_at[nears][threadIdx.x] = step * 8 + __ffs(near) - 1;
       }
       if (++in_bin == per || step + 1 == steps) {
         const double ta = warp_sum(sa);
@@ -836,19 +866,55 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
     }
     double mine = ra;  // the weight of this lane's bin
     if (kDraft && use_q) {
+      // a thread with more columns near the border than it notes: told by the sign of d
+      const bool many = __any_sync(0xffffffffu, !exact && nears > kNears);
       VerifySlot s;
       s.d = make_double2(warp_sum(a), warp_sum(d));
+      if (many) s.d.y = -s.d.y;
       const VerifySlot* all = exchange(s);
+      bool retake = false;
       a = d = 0.0;
       for (int i = lane; i < nslots; i += 32) {
         a += all[i].d.x;
-        d += all[i].d.y;
+        d += fabs(all[i].d.y);
+        retake |= all[i].d.y < 0.0;
       }
       a = warp_sum(a);
       d = warp_sum(d);
+      if (__any_sync(0xffffffffu, retake)) {
+        // columns of a common quotient, as where the rows agree but for a few
+        // columns: another pass with the sides by the exact sums
+        ratio = a / d;
+        exact = true;
+        continue;
+      }
       pinv = 1.0 / a;
       qinv = 1.0 / d;
-      mine = fmax(ra * pinv - rd * qinv, 0.0);
+      double fix = 0.0;  // of this lane's bin: what its near columns' true sides change
+      if (exact) nears = 0;
+#pragma unroll 1
+      for (int k = 0; __any_sync(0xffffffffu, k < nears); ++k) {
+        double change = 0.0;
+        int bin = 0;
+        if (k < nears) {
+          const int noted = near_at[k][threadIdx.x], step = noted >> 3;
+          const int x = group(step) * 8 - ps.shift + (noted & 7);
+          const double wp = exp2_64(
+              scale.log2_weight(__uint_as_float(scale.raise(__ldg(ps.src + x)) << 16)), table);
+          const double wq = exp2_64(
+              qscale.log2_weight(__uint_as_float(qscale.raise(__ldg(qs.src + x)) << 16)), table);
+          const double has = wp * pinv - wq * qinv;
+          change = fmax(has, 0.0) - (wp > wq * ratio ? has : 0.0);
+          bin = step / per;
+        }
+#pragma unroll 1
+        for (unsigned who = __ballot_sync(0xffffffffu, k < nears); who; who &= who - 1) {
+          const int from = __ffs(who) - 1;
+          const double c = __shfl_sync(0xffffffffu, change, from);
+          if (__shfl_sync(0xffffffffu, bin, from) == lane) fix += c;
+        }
+      }
+      mine = fmax(ra * pinv - rd * qinv + fix, 0.0);
     }
     VerifySlot s;
     s.d = make_double2(warp_sum(mine), 0.0);
@@ -861,8 +927,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
     const double incl = warp_scan(own, lane);
     const double total = __shfl_sync(0xffffffffu, incl, 31);
     if (kDraft && use_q && !exact && !(total > 0x1p-12)) {
-      // rows that almost agree: such roundings would count, so another pass with
-      // the sides by the exact sums
+      // rows that almost agree: the weights that near_border leaves out would
+      // count, so another pass with the sides by the exact sums
       ratio = a / d;
       exact = true;
       continue;
@@ -939,9 +1005,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   }
 }
 
+// Columns of a CTA of a cluster, in whole 16-byte groups.
+static int slice_of(int vocab, int ranks) { return ((vocab + ranks - 1) / ranks + 7) / 8 * 8; }
+
 static cudaError_t launch_cluster(void (*kernel)(VerifyParams), VerifyParams p, int batch, int ranks,
                                   bool dependent, cudaStream_t stream) {
-  p.slice = ((p.vocab + ranks - 1) / ranks + 7) / 8 * 8;
+  p.slice = slice_of(p.vocab, ranks);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
   cfg.blockDim = dim3(kVerifyThreads);
@@ -967,7 +1036,7 @@ static cudaError_t launch_cluster(void (*kernel)(VerifyParams), VerifyParams p, 
 constexpr int kWalkPerSm = 6, kDrawPerSm = 2;
 
 template <bool kDraft>
-static int launch_verify(const VerifyParams& p, int batch, cudaStream_t stream) {
+static int launch_verify(VerifyParams p, int batch, cudaStream_t stream) {
   static std::mutex mu;
   static bool done[64];
   int dev = 0;
@@ -992,9 +1061,11 @@ static int launch_verify(const VerifyParams& p, int batch, cudaStream_t stream) 
     return ranks;
   };
   const int ranks = fit(kWalkPerSm);
-  VerifyParams w = p;
-  w.ahead = static_cast<int64_t>(batch) * ranks <= kWalkPerSm * sms;
-  cudaError_t e = launch_cluster(verify_walk_kernel<kDraft>, w, batch, ranks, false, stream);
+  p.ahead = static_cast<int64_t>(batch) * ranks <= kWalkPerSm * sms;
+  // of a thread of the walk: whole groups in batches, then one at a slice's edge
+  const int groups = slice_of(p.vocab, ranks) / 8 + 1, step = kRowBatch * kVerifyThreads;
+  p.border = (groups + step - 1) / step + 1 <= kShortBatches ? kBorderShort : kBorderLong;
+  cudaError_t e = launch_cluster(verify_walk_kernel<kDraft>, p, batch, ranks, false, stream);
   if (e != cudaSuccess) return cuda_fail(e, "verify_walk_kernel launch");
   if (p.temperatures == nullptr) return NVATTN_OK;  // all greedy: nothing to draw
   e = launch_cluster(verify_draw_kernel<kDraft>, p, batch, fit(kDrawPerSm), true, stream);
