@@ -7,10 +7,17 @@
 // rounded on the way into the tensor cores but q (below) and the weights:
 // e4m3 converts to f16 exactly, so both products run as f16 MMAs with fp32
 // accumulation, the exponents are applied to the fp32 scores, and those of V
-// are folded into the softmax: with t_j the score in log2 units, the running
-// reference is M = max_j (t_j + kv_j), the weights given to the second product
-// are w_j = 2^(t_j + kv_j - M) <= 1 (one rounding, to f16: 2^-12), and the sum
-// runs over 2^(t_j - M). q's bf16 elements fit f16's 11 bits; its range is
+// are folded into the softmax: with t_j the score in log2 units, a warp's running
+// reference is M = max_j (t_j + max(kv_j, -80)) - 15, the weights given to the
+// second product are w_j = 2^(t_j + kv_j - M) <= 2^15, and the sum runs over
+// 2^(t_j - M). The weights are rounded to f16, half as wide as the plain form's
+// fp32: 2^-12 of a weight from 2^-29 of the reference's on (the 15 bits of f16's
+// range above one are for the rows whose V is small beside the largest row's, which
+// a single large channel can make: with w_j <= 1 they were off by 2^-12 only down to
+// 2^-14), 2^-40 of the reference's below that. The sum's terms lie within 2^-105 and
+// 2^95 of one for the keys that set M, so that neither rows of zeros (kv = -100)
+// overflow it nor values near bf16's largest (kv = 120) take it below fp32's range.
+// q's bf16 elements fit f16's 11 bits; its range is
 // brought in by a power of two a row, so only elements below 2^-14 of the
 // row's largest lose bits (2^-25 of it).
 //
@@ -46,6 +53,10 @@ constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
 // 6 x 2 91, 3 x 4 92, 2 x 6 94.
 constexpr int dec8_warps(int) { return 4; }
 constexpr int dec8_ctas(int NB) { return NB == 1 ? 3 : 2; }
+
+// The softmax's reference (top of the file): V exponents count from the first on, and
+// the largest weight is 2^ the second.
+constexpr float kLowestRef8 = -80.f, kHeadroom8 = 15.f;
 
 // Shared memory of one warp: its K and V tile, their exponent bytes.
 constexpr int kWarpBytes8 = 2 * kTile8;
@@ -328,11 +339,12 @@ __global__ void __launch_bounds__(dec8_warps(NB) * 32, dec8_ctas(NB))
         float mx = neg_inf();
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
-          mx = fmax3(mx, s[mt][nb][j] + ve[mt][0], s[mt][nb][2 + j] + ve[mt][1]);
+          mx = fmax3(mx, s[mt][nb][j] + fmaxf(ve[mt][0], kLowestRef8),
+                     s[mt][nb][2 + j] + fmaxf(ve[mt][1], kLowestRef8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        mn[nb][j] = fmaxf(m[nb][j], mx);
+        mn[nb][j] = fmaxf(m[nb][j], mx - kHeadroom8);
         grew |= mn[nb][j] > m[nb][j];
       }
     }
