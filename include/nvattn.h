@@ -310,7 +310,7 @@ NVATTN_API int nvattn_paged_decode_fp8(
  * its own pages alone. shared_len is a multiple of block_size (0: none shared),
  * block_size one of 128. k_scale and v_scale NULL: bf16 caches; otherwise fp8
  * caches as for nvattn_paged_decode_fp8. q rows are 16-byte aligned; tables
- * cover up to 2^30 keys.
+ * cover up to 2^30 keys; softmax_scale is finite and > 0.
  *
  * `workspace` (device, 256-byte aligned, >= nvattn_shared_prefix_workspace_bytes
  * of the same sizes; fp8 = 0 or 1) holds fp32 partials of both parts and, for an

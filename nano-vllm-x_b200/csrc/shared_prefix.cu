@@ -15,6 +15,7 @@
 // the workspace first: it is read once by that, and the tensor-core kernel
 // takes it from L2.
 #include <algorithm>
+#include <cmath>
 
 #include "decode.cuh"
 #include "shared_prefix.cuh"
@@ -124,6 +125,9 @@ extern "C" int nvattn_shared_prefix_decode(
     return fail(NVATTN_ERR_UNSUPPORTED, msg("block_size must be a multiple of 128"));
   if (shared_len < 0 || shared_len % block_size || shared_len / block_size > max_blocks_per_seq)
     return fail(NVATTN_ERR_INVALID, msg("shared_len must be whole blocks of the table"));
+  // the tensor-core pass takes the maximum of the scores before it scales them
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return fail(NVATTN_ERR_INVALID, msg("softmax_scale must be finite and > 0"));
   if (!aligned16(q) || (q_stride_tok * 2) % 16 || (q_stride_head * 2) % 16)
     return fail(NVATTN_ERR_UNSUPPORTED, msg("q base and strides must be 16-byte multiples (TMA)"));
   const SharedLayout w = shared_layout(batch, num_heads, num_kv_heads, max_blocks_per_seq,

@@ -574,8 +574,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     block_table (whatever row 0's own length), read once for the whole batch; keys
     behind them come through each sequence's own row. cache_seqlens counts all keys; a row with fewer
     than shared_len (0: padding, zeros) is attended over its own row alone.
-    shared_len must be whole blocks, block_size a multiple of 128. With
-    k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
+    shared_len must be whole blocks, block_size a multiple of 128, softmax_scale
+    > 0. With k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
     ``workspace``: uint8, ``shared_prefix_workspace_bytes`` of the same sizes.
     """
     dev = _one_device(q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out,
