@@ -596,6 +596,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     batch, num_heads, head_dim, out = _check_decode(q, out, cache_seqlens, block_table,
                                                     num_kv_heads, d)
     shared_len, max_blocks = int(shared_len), block_table.shape[1]
+    if batch and not 0 <= shared_len <= max_blocks * block_size:  # it is cut to 32 bits below
+        raise ValueError("shared_len must be whole blocks of the table")
     with _on_device(dev):
         ws_ptr, ws_bytes, _ws = _workspace(
             _workspace_bytes(dev, "nvattn_shared_prefix_workspace_bytes", batch, num_heads,
