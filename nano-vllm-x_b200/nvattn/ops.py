@@ -241,6 +241,8 @@ def _workspace(need: int, workspace: torch.Tensor | None, like: torch.Tensor):
         return None, 0, None
     if workspace is None:
         workspace = like.new_empty(need, dtype=torch.uint8)
+    elif not workspace.is_contiguous():  # fewer bytes behind its pointer than it has elements
+        raise ValueError("workspace must be contiguous")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
