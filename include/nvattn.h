@@ -477,12 +477,13 @@ NVATTN_API int nvattn_sample_merge(const uint64_t* keys, int64_t num_shards, int
  * and where a node has no child the next token is drawn from p. Either way the
  * tokens follow the target's law. The draw takes the first column whose
  * cumulative weight exceeds u_pick[b] * total, in column order; where rounding
- * leaves no weight it is from p. temperatures NULL or <= 0: greedy, a child is
- * accepted iff its token is the argmax (first index on ties), which is also the
- * draw (above 1e30 they count as 1e30). NaN and -inf logits have no probability, an infinite one all of it; a
- * row with nothing else accepts nothing and gives column 0. A probability below
- * 2^-950 of its row's largest counts as none. A drafted token
- * outside [0, vocab) is rejected. Decisions are those of 64-bit arithmetic.
+ * leaves no weight it is from p. temperatures NULL, <= 0 or NaN: greedy, a
+ * child is accepted iff its token is the argmax (first index on ties), which is
+ * also the draw (above 1e30 they count as 1e30). NaN and -inf logits have no
+ * probability, an infinite one all of it; a row with nothing else accepts
+ * nothing and gives column 0. A probability below 2^-950 of its row's largest
+ * counts as none. A drafted token outside [0, vocab) is rejected. Decisions are
+ * those of 64-bit arithmetic, up to the rounding of its sums.
  *
  * out_num[b] = number of accepted drafts a; out_path[b][0..a] = the walked
  * nodes from 0; out_tokens[b][0..a-1] = the accepted tokens, out_tokens[b][a] =

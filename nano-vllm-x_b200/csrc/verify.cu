@@ -83,6 +83,12 @@ struct VerifyParams {
   int32_t* out_num;
 };
 
+// A sequence's temperature, up to kMaxTemperature; 0 for greedy, NaN among it.
+__device__ __forceinline__ float temperature_of(const VerifyParams& p, int b) {
+  const float t = p.temperatures ? p.temperatures[b] : 0.f;
+  return t > 0.f ? fminf(t, kMaxTemperature) : 0.f;
+}
+
 // What a warp tells the cluster: (max, sum) of its part of the target's and the
 // draft's row; or a pick key; or two fp64 sums.
 union VerifySlot {
@@ -493,7 +499,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_walk_kernel(const Ve
   const int x0 = min(rank * p.slice, p.vocab);
   const int len = min(p.slice, p.vocab - x0);
   const int n = p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
-  const float temp = p.temperatures ? fminf(p.temperatures[b], kMaxTemperature) : 0.f;
+  const float temp = temperature_of(p, b);
   const bool greedy = !(temp > 0.f);
   const double c64 = greedy ? 1.0 : 1.4426950408889634074 / static_cast<double>(temp);
   const float c32 = fminf(static_cast<float>(c64), 1e30f);
@@ -725,7 +731,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_draw_kernel(const Ve
   fill_table(table);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the walk is done
   const int n = p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
-  const float temp = p.temperatures ? fminf(p.temperatures[b], kMaxTemperature) : 0.f;
+  const float temp = temperature_of(p, b);
   const int num = p.out_num[b];
   cg::this_cluster().sync();  // all have read num, and run
   exchange.started = true;

@@ -868,7 +868,7 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: tor
     from; without them the drafts count as proposed with certainty (greedy or
     n-gram drafts). ``u_accept`` (B, n - 1) and ``u_pick`` (B,) are uniform
     random numbers in [0, 1), fp32. ``temperatures`` (B,) fp32 as in ``sample``
-    (<= 0 or None: greedy). ``num_nodes`` (B,) int32: nodes in use per sequence
+    (<= 0, NaN or None: greedy). ``num_nodes`` (B,) int32: nodes in use per sequence
     (0: a padding row).
 
     Returns (tokens (B, n) int64: the accepted tokens, then the drawn one, then
