@@ -255,10 +255,9 @@ NVATTN_API int nvattn_paged_decode_noalloc(const void* q, int64_t q_stride_tok, 
  * nvattn_varlen_prefill takes (exactly: elements times 2^k): sequence b's key
  * j goes to row cu_seqlens_k[b] + j of k_out and v_out [total_k]
  * [num_kv_heads][128]. Rows outside [cu_seqlens_k[0], cu_seqlens_k[num_seqs])
- * are left as they were, or zeroed with zero_rest != 0 (a dense prefill reads
- * up to 127 rows behind a sequence's keys, masked: they must be finite); keys
- * whose block id or table column is out of range
- * become zeros and set NVATTN_STATUS_BAD_BLOCK. cu_seqlens_k must not decrease.
+ * are left as they were, or zeroed with zero_rest != 0; keys whose block id or
+ * table column is out of range become zeros and set NVATTN_STATUS_BAD_BLOCK.
+ * cu_seqlens_k must not decrease.
  * num_seqs 0: nothing is written.
  *
  * nvattn_paged_decode_fp8 is nvattn_paged_decode over these caches, with the

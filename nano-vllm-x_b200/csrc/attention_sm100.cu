@@ -34,9 +34,9 @@
 // Masks (query token i of the sequence, key j):
 //   causal (dense/paged): j <= seqlen_k - seqlen_q + i   (bottom-right aligned)
 //   tree: j < context_len, or bit (j - context_len) of the row's mask word.
-// Keys past the sequence's end in the last tile of the paged cache are stale
-// bytes (maybe NaN): their scores are masked and their V rows zeroed in
-// shared memory before the P V product.
+// Keys past the sequence's end in the last tile are stale bytes of a paged cache,
+// or in dense K/V the next sequence's rows (maybe NaN either way): their scores are
+// masked and their V rows zeroed in shared memory before the P V product.
 // Query rows past the sequence (the last row block, short drafts) are never
 // written: a warp with no valid row skips its softmax entirely, and inside a
 // live warp such rows take the unmasked path (rows are independent in both
@@ -141,6 +141,21 @@ __device__ __forceinline__ uint64_t vdesc(uint32_t base, int kk) {
   // MN-major V: 16-key step kk starts at row 16*kk; the two 64-dim halves are
   // kHalf apart (leading byte offset), 8-row groups 1024 B apart (stride).
   return sm100::sw128_desc(base + kk * 16 * 128, kHalf, 1024);
+}
+
+// Dense K/V: zeroes rows left..127 of a V tile, which are the next sequence's (maybe
+// not finite), so that 0 * NaN cannot reach O; thread r of a warpgroup, row r. A call
+// and not inlined: in the softmax loop its registers cost every tile (8 x 2048 tokens,
+// 32/8 heads: 347 us, inlined 358, without it 350).
+__device__ __noinline__ void zero_rows_behind(uint8_t* v, int left, int r, uint64_t* full,
+                                              uint32_t parity) {
+  __all_sync(0xffffffffu, mbar_wait(full, parity));
+  if (r >= left) {
+    int4* vrow = reinterpret_cast<int4*>(v + r * 128);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) vrow[c] = vrow[c + kHalf / 16] = make_int4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
 }
 
 template <int MODE>
@@ -453,6 +468,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       sm100::fence_after_sync();
       const int j0 = (jb + j) * kBN;
+      if (MODE == kDense && wg == 0 && j == ntiles - 1) {
+        const int left = p.cu_k[b + 1] - p.cu_k[b] - j0;  // read again: a register less
+        if (left < kBN)  // V_j lands just behind the K_j that S_j came from
+          zero_rows_behind(smem + kQBytes + (j % kStages) * 2 * kOperand + kOperand, left, r,
+                           &bars->v_full[j % kStages], (j / kStages) & 1);
+      }
       if (!warp_live) {
         if (MODE != kDense && wg == 0 && j == ntiles - 1 && kend - j0 < kBN) {
           const int vlim = kend - j0;
