@@ -124,11 +124,12 @@ class Attention(nn.Module):
         """Prefix-cache prefill over an fp8 cache: the sequences' rows read back, then dense.
 
         The rows' number is on the device only, so each group of sequences gets
-        room for max_seqlen_k (or a full table) apiece: ragged batches would
-        claim many times their keys if all were read back at once.
+        room for max_seqlen_k apiece: ragged batches would claim many times their
+        keys if all were read back at once. (A sequence may have one key more than
+        its table, so that its length is flagged.)
         """
         table, cu_q, cu_k = context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k
-        longest = max(1, min(context.max_seqlen_k, table.shape[1] * self.k_cache.shape[1]))
+        longest = max(1, min(context.max_seqlen_k, table.shape[1] * self.k_cache.shape[1] + 1))
         step = max(1, READ_BACK_KEYS // longest)
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         for b in range(0, table.shape[0], step):
