@@ -126,18 +126,21 @@ class Attention(nn.Module):
         The rows' number is on the device only, so each group of sequences gets
         room for max_seqlen_k apiece: ragged batches would claim many times their
         keys if all were read back at once. (A sequence may have one key more than
-        its table, so that its length is flagged.)
+        its table, so that its length is flagged.) Rows behind the keys are left as
+        they are: the prefill takes nothing from them.
         """
         table, cu_q, cu_k = context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k
         longest = max(1, min(context.max_seqlen_k, table.shape[1] * self.k_cache.shape[1] + 1))
         step = max(1, READ_BACK_KEYS // longest)
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k, v = q.new_empty((2, min(step, table.shape[0]) * longest, *self.k_cache.shape[2:])).unbind()
         for b in range(0, table.shape[0], step):
             rows = table[b:b + step]
+            n = rows.shape[0] * longest
             ck = cu_k[b:b + step + 1]
             ck = ck - ck[0]
-            k, v = ops.load_kvcache_fp8(self.k_cache, self.v_cache, self.k_scale, self.v_scale,
-                                        ck, rows, rows.shape[0] * longest)
-            ops.varlen_prefill(q, k, v, cu_q[b:b + step + 1], ck, context.max_seqlen_q,
+            ops.load_kvcache_fp8(self.k_cache, self.v_cache, self.k_scale, self.v_scale, ck, rows, n,
+                                 k[:n], v[:n])
+            ops.varlen_prefill(q, k[:n], v[:n], cu_q[b:b + step + 1], ck, context.max_seqlen_q,
                                context.max_seqlen_k, softmax_scale=self.scale, causal=True, out=o)
         return o
