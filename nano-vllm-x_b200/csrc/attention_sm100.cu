@@ -448,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int hh = r % group;
     const bool valid = r < p.rpt && tok < Lq &&
                        (MODE != kShared || p.seqlens[tok] >= p.shared_len);
-    const int lim = valid ? ((MODE != kTree && MODE != kShared && p.causal) ? min(Lk - 1, diag + tok) : Lk - 1) : -1;
+    const bool bottom_right = MODE != kTree && MODE != kShared && p.causal;
+    const int lim = valid ? (bottom_right ? min(Lk - 1, diag + tok) : Lk - 1) : -1;
     uint64_t mword = 0;
     if (MODE == kTree && valid) mword = p.tree_mask[q_begin + tok];
     // first key index at which this row needs masking

@@ -86,8 +86,8 @@ int check_decode_args(const char* who, const void* q, int64_t q_stride_tok, int6
                       int64_t block_table_stride, int32_t max_blocks_per_seq, int32_t num_blocks,
                       int32_t block_size, int32_t batch, int32_t num_heads, int32_t num_kv_heads,
                       int32_t head_dim);
-// The suffix kernels over p's own keys; after_prefix: as programmatic
-// dependents of the prefix's kernel, launched just before on `stream`.
+// The suffix kernels over p's own keys, as programmatic dependents of the prefix's
+// kernel, launched just before on `stream` (bf16: if after_prefix).
 int launch_decode_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache, int batch,
                          bool after_prefix, cudaStream_t stream);
 // All keys of every row, merged into p.out.
@@ -96,7 +96,7 @@ int launch_decode_fp8_whole(const DecodeParams& p, const void* k_cache, const vo
                             cudaStream_t stream);
 int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
-                             bool after_prefix, cudaStream_t stream);
+                             cudaStream_t stream);
 // Checks an fp8 cache's scale pointers.
 int check_fp8_scales(const char* who, const void* k_scale, const void* v_scale);
 // Key positions are 32-bit: a table may cover up to 2^30 keys.

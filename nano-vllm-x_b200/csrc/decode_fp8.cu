@@ -25,16 +25,18 @@
 // sequences of 100 to 2048 keys, 16/8 heads: 88 us, 6.1 TB/s, 0.93 of a copy's
 // rate; 32 sequences of 4k to 32k keys, 64/8 heads: 177 us, 6.0 TB/s). What is
 // left to hide is the arithmetic around the products, so the keys are the M rows
-// of the MMAs and the query heads the 8 columns (S^T = K Q^T, O^T = V^T W^T): with up to 8 heads a group no MMA row and no softmax lane is
-// padding, and the conversions (2 a 4-byte word, plus one byte permute for V)
-// serve all heads. A warp owns whole 64-key tiles, the warps of a CTA taking
-// turns, so maxima, barrier waits and rescales are paid once for 64 keys. Each
-// warp is its own producer: it has room for one tile of K and one of V, and
-// sends for the next tile's K as soon as the scores are out and for its V as
-// soon as the second product is, so that either half is in flight while the
-// warp works on the other. Up to 8 consecutive splits of a row form a cluster,
-// whose CTAs merge through each other's shared memory: with no more splits than
-// that the output is written at once, otherwise one fp32 partial a cluster.
+// of the MMAs and the query heads the 8 columns (S^T = K Q^T, O^T = V^T W^T): inside
+// a tile no key is padding, and the conversions (2 a 4-byte word, plus one byte
+// permute for V) serve all heads. Columns, and the quad lanes that own them, are
+// padding where the heads a KV head are no multiple of 8 (6 of 8 with 2 heads). A
+// warp owns whole 64-key tiles, the warps of a CTA taking turns, so maxima, barrier
+// waits and rescales are paid once for 64 keys. Each warp is its own producer: it
+// has room for one tile of K and one of V, and sends for the next tile's K as soon
+// as the scores are out and for its V as soon as the second product is, so that
+// either half is in flight while the warp works on the other. Up to 8 consecutive
+// splits of a row form a cluster, whose CTAs merge through each other's shared
+// memory: with no more splits than that the output is written at once, otherwise
+// one fp32 partial a cluster.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -51,7 +53,7 @@ constexpr int kTile8 = kTile * kHeadDim;      // one 64-key e4m3 tile (8 KB)
 // Warps of a CTA and CTAs of an SM for NB blocks of 8 query heads (registers a
 // thread grow with NB). 256 sequences of 100 to 2048 keys: 4 warps x 3 CTAs 88 us;
 // 6 x 2 91, 3 x 4 92, 2 x 6 94.
-constexpr int dec8_warps(int) { return 4; }
+constexpr int kDec8Warps = 4;
 constexpr int dec8_ctas(int NB) { return NB == 1 ? 3 : 2; }
 
 // The softmax's reference (top of the file): V exponents count from the first on, and
@@ -62,7 +64,7 @@ constexpr float kLowestRef8 = -80.f, kHeadroom8 = 15.f;
 constexpr int kWarpBytes8 = 2 * kTile8;
 constexpr int kWarpScales8 = 2 * kTile;
 constexpr int dec8_smem(int NB) {
-  return dec8_warps(NB) * (kWarpBytes8 + kWarpScales8 + 2 * 8 + 8 * NB * 8) + 8 * NB * 8 + 1024;
+  return kDec8Warps * (kWarpBytes8 + kWarpScales8 + 2 * 8 + 8 * NB * 8) + 8 * NB * 8 + 1024;
 }
 static_assert(16 * kOPad * 4 <= kWarpBytes8, "the merge buffer reuses the tiles");
 
@@ -152,12 +154,12 @@ __device__ __forceinline__ float load_q8(const __nv_bfloat16* row, bool live, in
 // p.key_begin on, as fp32 partials for the merge with the keys before
 // (shared_prefix.cu).
 template <int NB, bool kSuffix>
-__global__ void __launch_bounds__(dec8_warps(NB) * 32, dec8_ctas(NB))
+__global__ void __launch_bounds__(kDec8Warps * 32, dec8_ctas(NB))
     paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap,
                             const uint8_t* __restrict__ k_scale,
                             const uint8_t* __restrict__ v_scale, const DecodeParams p) {
-  constexpr int kWarps = dec8_warps(NB);
+  constexpr int kWarps = kDec8Warps;
   const int split = blockIdx.x;
   const int g = blockIdx.y;
   const int b = blockIdx.z;
@@ -637,7 +639,7 @@ static int raise_smem8() {
 template <int NB, bool kSuffix>
 static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
-                             bool after_prefix, cudaStream_t stream) {
+                             cudaStream_t stream) {
   CUtensorMap kmap, vmap;
   int rc = make_cache8_map(&kmap, k_cache, p.num_blocks, p.block_size, p.num_kv_heads);
   if (rc) return rc;
@@ -647,7 +649,7 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.nsplit, p.num_kv_heads, batch);
-  cfg.blockDim = dim3(dec8_warps(NB) * 32);
+  cfg.blockDim = dim3(kDec8Warps * 32);
   cfg.dynamicSmemBytes = dec8_smem(NB);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -657,7 +659,7 @@ static int launch_decode_fp8(const DecodeParams& p, const void* k_cache, const v
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = after_prefix ? 2 : 1;
+  cfg.numAttrs = kSuffix ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_fp8_kernel<NB, kSuffix>, kmap, vmap,
                                            k_scale, v_scale, p);
   return e == cudaSuccess ? NVATTN_OK : cuda_fail(e, "paged_decode_fp8 launch");
@@ -667,20 +669,19 @@ int launch_decode_fp8_whole(const DecodeParams& p, const void* k_cache, const vo
                             const uint8_t* k_scale, const uint8_t* v_scale, int batch,
                             cudaStream_t stream) {
   const int rc = p.group <= 8 ? launch_decode_fp8<1, false>(p, k_cache, v_cache, k_scale, v_scale,
-                                                            batch, false, stream)
+                                                            batch, stream)
                               : launch_decode_fp8<2, false>(p, k_cache, v_cache, k_scale, v_scale,
-                                                            batch, false, stream);
+                                                            batch, stream);
   if (rc || p.nsplit == p.cluster) return rc;
   return launch_merge_partials(p, nullptr, nullptr, 0, batch, stream);
 }
 
 int launch_decode_fp8_suffix(const DecodeParams& p, const void* k_cache, const void* v_cache,
                              const uint8_t* k_scale, const uint8_t* v_scale, int batch,
-                             bool after_prefix, cudaStream_t stream) {
-  return p.group <= 8 ? launch_decode_fp8<1, true>(p, k_cache, v_cache, k_scale, v_scale, batch,
-                                                   after_prefix, stream)
-                      : launch_decode_fp8<2, true>(p, k_cache, v_cache, k_scale, v_scale, batch,
-                                                   after_prefix, stream);
+                             cudaStream_t stream) {
+  return p.group <= 8
+             ? launch_decode_fp8<1, true>(p, k_cache, v_cache, k_scale, v_scale, batch, stream)
+             : launch_decode_fp8<2, true>(p, k_cache, v_cache, k_scale, v_scale, batch, stream);
 }
 
 // Splits of a row, in 64-key tiles: the largest of 32/16/8/4 that gives 8 CTAs

@@ -205,7 +205,7 @@ extern "C" int nvattn_shared_prefix_decode(
   const bool after = w.np > 0;
   if (fp8 && !after)
     return launch_decode_fp8_whole(p, k_cache, v_cache, k_scale, v_scale, batch, s);
-  rc = fp8 ? launch_decode_fp8_suffix(p, k_cache, v_cache, k_scale, v_scale, batch, after, s)
+  rc = fp8 ? launch_decode_fp8_suffix(p, k_cache, v_cache, k_scale, v_scale, batch, s)
            : launch_decode_suffix(p, k_cache, v_cache, batch, after, s);
   if (rc) return rc;
   return launch_merge_partials(p, prefix_o, prefix_ml, w.np, batch, s);

@@ -368,7 +368,7 @@ struct RowSum {
 
 // This thread's part of a slice of one row (kRowBatch vectors in flight), or of
 // the target's and the draft's row together (that many of each).
-constexpr int kRowBatch = 5, kRowBatch2 = 5;
+constexpr int kRowBatch = 5;
 
 // The partial groups of a slice, one on each of two threads.
 __device__ __forceinline__ int edge_group(const Slice& s) {
@@ -379,16 +379,15 @@ __device__ __forceinline__ int edge_group(const Slice& s) {
 template <bool kTwo>
 __device__ __forceinline__ void scan_rows(const Slice& s, const Slice& s2, float c, RowSum& r,
                                           RowSum& r2) {
-  constexpr int kBatch = kTwo ? kRowBatch2 : kRowBatch;
   const int hi = kTwo ? max(s.hi, s2.hi) : s.hi;
 #pragma unroll 1
-  for (int g0 = threadIdx.x; g0 < hi; g0 += kBatch * kVerifyThreads) {
-    uint32_t w[kBatch][4], v[kTwo ? kBatch : 1][4];
+  for (int g0 = threadIdx.x; g0 < hi; g0 += kRowBatch * kVerifyThreads) {
+    uint32_t w[kRowBatch][4], v[kTwo ? kRowBatch : 1][4];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) s.load(g0 + u * kVerifyThreads, w[u]);
+    for (int u = 0; u < kRowBatch; ++u) s.load(g0 + u * kVerifyThreads, w[u]);
     if constexpr (kTwo) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) s2.load(g0 + u * kVerifyThreads, v[u]);
+      for (int u = 0; u < kRowBatch; ++u) s2.load(g0 + u * kVerifyThreads, v[u]);
     }
     r.add(w, c);
     if constexpr (kTwo) r2.add(v, c);
