@@ -262,9 +262,10 @@ NVATTN_API int nvattn_paged_decode_noalloc(const void* q, int64_t q_stride_tok, 
  *
  * nvattn_paged_decode_fp8 is nvattn_paged_decode over these caches, with the
  * same sizes and limits (and tables of up to 2^30 keys) and a workspace of
- * nvattn_decode_fp8_workspace_bytes (0 for short tables: NULL will do); scores
- * and sums are fp32 and the output is rounded to bf16 once. Scales must be
- * 16-byte aligned.
+ * nvattn_decode_fp8_workspace_bytes (0 for short tables: NULL will do). Scores
+ * and sums are fp32; a key's weight times 2^(its V exponent) goes to the tensor
+ * cores as f16 (2^-12 of it, from 2^-29 of the largest on); the output is
+ * rounded to bf16 once. Scales must be 16-byte aligned.
  */
 NVATTN_API int nvattn_store_kvcache_fp8(const void* key, int64_t key_stride, const void* value,
                                         int64_t value_stride, void* k_cache, void* v_cache,
@@ -309,7 +310,11 @@ NVATTN_API int nvattn_paged_decode_fp8(
  * its own pages alone. shared_len is a multiple of block_size (0: none shared),
  * block_size one of 128. k_scale and v_scale NULL: bf16 caches; otherwise fp8
  * caches as for nvattn_paged_decode_fp8. q rows are 16-byte aligned; tables
- * cover up to 2^30 keys; softmax_scale is finite and > 0.
+ * cover up to 2^30 keys; softmax_scale is finite and > 0. Scores and sums are
+ * fp32; weights go to the tensor cores as bf16 (2^-8 of a weight), except those
+ * of an fp8 cache's own keys, and of all its keys where the prefix is read once
+ * a row (batch * shared_len * num_kv_heads * 258 bytes up to 64 MB), which are
+ * rounded as in nvattn_paged_decode_fp8.
  *
  * `workspace` (device, 256-byte aligned, >= nvattn_shared_prefix_workspace_bytes
  * of the same sizes; fp8 = 0 or 1) holds fp32 partials of both parts and, for an

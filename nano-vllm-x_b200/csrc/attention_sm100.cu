@@ -48,7 +48,11 @@
 // CTA writes fp32 partials of its split of the keys. Tensor- and softmax-bound
 // like the prefill: 2.2 us a tile of 256 rows x 128 keys, and about 11 us to
 // start and to write the partials (16,384 keys, 512 rows for each of 8 KV heads:
-// 45 us, 0.76 PFLOP/s).
+// 45 us, 0.76 PFLOP/s). Its roundings are the prefill's: weights go to the tensor
+// cores as bf16, like V (one type for both operands; 2^-8 of a weight, with random
+// sign over the keys), and one exponential in four is a cubic of 7.5e-5, a fiftieth of
+// that. Outputs are then 0.0023 from 64 bits (root mean square, relative) where
+// fp32 weights would leave the output's own rounding, 0.0017.
 #include <algorithm>
 #include <cmath>
 #include <mutex>

@@ -38,7 +38,17 @@ struct SharedLayout {
 // 64 MB: 15.7 and 21.2), with an fp8 cache, whose prefix is expanded first, from
 // 64 MB on (16 rows of 1024, 32 MB: 17.7 and 11.9; 32/8 heads, 32 rows of 1024, 64
 // MB: 20.4 and 20.3; 64 rows of 1024: 25.3 and 32.8). Otherwise the decode kernel
-// takes all keys of a row, the shared pages from row 0 of the table.
+// takes all keys of a row, the shared pages from row 0 of the table. The tensor work
+// grows with the heads a KV head, and the cost of a row's own reads with it: at 1, 8
+// and 16 heads a KV head the bf16 sides cross at the same bytes (8 rows of 1024 over 8
+// KV heads: 11.8 and 12.2, 13.8 and 14.6, 14.1 and 17.2; half as many: 12.3 and 10.1
+// with 8), the fp8 sides too with 1 and 8 (32 rows of 512: 17.6 and 14.7, 21.4 and
+// 20.1) and at half of them with 16 (16 rows of 1024: 22.4 and 24.4).
+// The two sides round differently. Read once a row, a bf16 cache's weights go to the
+// tensor cores as bf16 (decode.cu) and an fp8 cache's as f16 (decode_fp8.cu: 0.0017
+// from 64 bits, the output's own rounding); the prefix apart takes bf16 weights
+// against the bf16 values of either cache (0.0023), its own keys as before. So an fp8
+// caller's batch that grows past the rule keeps 2^-8 of a weight instead of 2^-12.
 static bool prefix_apart(int batch, int num_kv_heads, int shared_len, bool fp8) {
   const int64_t keys = static_cast<int64_t>(batch) * shared_len * num_kv_heads;
   return fp8 ? keys * 258 > (64 << 20) : keys * 512 > (32 << 20);

@@ -22,21 +22,25 @@
 // exponential and about three other instructions a logit (each thread sums
 // against its own maximum) and one cluster barrier: every warp writes its sums
 // into the shared memory of all CTAs, and after the barrier every warp adds the
-// same numbers up and takes the same decision, with nothing to broadcast. Rows
-// are a chain, bound by latency (about 5 us a node alone, 7 beside 63 other
-// sequences): the next node's rows are sent for to L2 before it is accepted, and
-// the code of a step is kept short (it once overran the instruction cache at
-// twice the time). The draw then goes over each sequence's last row, all
-// sequences at once. 64 sequences of 7 drafts, 151,936 columns: walk 75 us, draw
-// 46; both in one kernel, where an early end is drawn at once, take the same 120,
-// and so does a step that sums up a node's and its first child's rows together
-// (130) or a table of weights over the rows' bf16 values for the draw (121).
+// same numbers up and takes the same decision, with nothing to broadcast. The walk
+// takes a node's rows after the decision that leads there, so only rows on the path
+// are read, but one after another: it is bound by latency (about 5 us a node alone, 7
+// beside 63 other sequences). That is this walk's order, not the operator's: the
+// sums of all rows could be taken at once and the decisions after. The next node's
+// rows are sent for to L2 before it is accepted, and the code of a step is kept short
+// (it once overran the instruction cache at twice the time). The draw then goes over
+// each sequence's last row, all sequences at once, in fp64 throughout, which an
+// answer clear of its border does not need. 64 sequences of 7 drafts, 151,936
+// columns: walk 75 us, draw 49 (46 before it noted the columns near the residual's
+// border; then both in one kernel, where an early end is drawn at once, took the same
+// 120, a step that sums up a node's and its first child's rows together 130, a table
+// of weights over the rows' bf16 values for the draw 121).
 //
 // The answers are tokens, so sums that decide between neighbours are kept in
 // 64 bits: the draw's cumulative weights always (with 151,936 weights of which
 // many are near 1e-6, sums in fp32 would move a border past u in about one
-// draw in a hundred), an acceptance when the fp32 sums leave its outcome
-// within 2^-14 of the border. 2^t in fp64 is table-driven (P. T. P. Tang, ACM
+// draw in a hundred), the sides of max(p - q, 0) where the fp32 sums leave them
+// open, an acceptance when they leave its outcome within 2^-14 of the border. 2^t in fp64 is table-driven (P. T. P. Tang, ACM
 // TOMS 15(2), 1989): t = k/1024 + f, |f| <= 2^-11, 2^t = 2^(k>>10) *
 // T[k & 1023] * 2^f with a cubic (error (f ln 2)^4/24 < 6e-16), 8 fp64
 // operations, which bound the draw. In it a warp owns consecutive columns, its
