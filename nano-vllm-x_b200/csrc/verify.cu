@@ -40,12 +40,12 @@
 // 64 bits: the draw's cumulative weights always (with 151,936 weights of which
 // many are near 1e-6, sums in fp32 would move a border past u in about one
 // draw in a hundred), the sides of max(p - q, 0) where the fp32 sums leave them
-// open, an acceptance when they leave its outcome within 2^-14 of the border. 2^t in fp64 is table-driven (P. T. P. Tang, ACM
-// TOMS 15(2), 1989): t = k/1024 + f, |f| <= 2^-11, 2^t = 2^(k>>10) *
-// T[k & 1023] * 2^f with a cubic (error (f ln 2)^4/24 < 6e-16), 8 fp64
-// operations, which bound the draw. In it a warp owns consecutive columns, its
-// lanes keep the sums of consecutive bins, and prefix sums over warps, bins and
-// lanes find the column.
+// open, an acceptance when they leave its outcome within 2^-14 of the border. 2^t
+// in fp64 is table-driven (P. T. P. Tang, ACM TOMS 15(2), 1989): t = k/1024 + f,
+// |f| <= 2^-11, 2^t = 2^(k>>10) * T[k & 1023] * 2^f with a cubic (error
+// (f ln 2)^4/24 < 6e-16), 8 fp64 operations, whose latency bounds the draw. In it
+// a warp owns consecutive columns, its lanes keep the sums of consecutive bins, and
+// prefix sums over warps, bins and lanes find the column.
 #include <cooperative_groups.h>
 
 #include <mutex>
