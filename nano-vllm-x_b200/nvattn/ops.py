@@ -535,7 +535,8 @@ def paged_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_decode`` over an fp8 cache (``store_kvcache_fp8``); q, out: (B, H, d) bf16.
 
-    ``workspace``: uint8, ``decode_fp8_workspace_bytes`` of the same sizes.
+    ``workspace``: contiguous uint8, ``decode_fp8_workspace_bytes`` of the same
+    sizes, for one call at a time.
     """
     dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, out,
                       workspace)
@@ -578,7 +579,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     than shared_len (0: padding, zeros) is attended over its own row alone.
     shared_len must be whole blocks, block_size a multiple of 128, softmax_scale
     > 0. With k_scale/v_scale the caches are fp8 (``store_kvcache_fp8``).
-    ``workspace``: uint8, ``shared_prefix_workspace_bytes`` of the same sizes.
+    ``workspace``: contiguous uint8, ``shared_prefix_workspace_bytes`` of the same
+    sizes, for one call at a time.
     """
     dev = _one_device(q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out,
                       workspace)
@@ -874,7 +876,8 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, u_accept: tor
     Returns (tokens (B, n) int64: the accepted tokens, then the drawn one, then
     -1; path (B, n) int32: the walked nodes from 0, then -1, for
     ``tree.compaction_moves``; accepted (B,) int32). The tokens follow the
-    target's law; every decision is that of 64-bit arithmetic.
+    target's law; every decision is that of 64-bit arithmetic, up to the rounding
+    of its sums.
     """
     dev = _one_device(logits, draft_tokens, u_accept, u_pick, temperatures, draft_logits, parents,
                       num_nodes)
